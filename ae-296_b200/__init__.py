@@ -11,6 +11,7 @@ from .ops import (LoraBatch, LoraPlan, LoraWorkspace, add_lora_bgmv, add_lora_bg
                   add_lora_bgmv_static, add_lora_bgmv_static_status, add_lora_bgmv_v2, add_lora_sgmv,
                   add_lora_bgmv_workspace_bytes, adapters_of, apply, invalidate_plan_cache)
 from . import ops                                            # noqa: F401
+from .decode import append_kv, int4_linear, prefix_attention   # noqa: F401
 from .lora_gpu import Lora_GPU                               # noqa: F401
 from .lora_cpu import Lora_CPU, ShmSegments                  # noqa: F401
 from .placement import place_by_adapter                      # noqa: F401

@@ -47,6 +47,32 @@ class Proj(C.Structure):
                 ("ldx", C.c_int64), ("ldy", C.c_int64), ("h_in", C.c_int32), ("h_out", C.c_int32)]
 
 
+class KvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class Append(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("q_out", "q", "k", "v", "dq", "dk", "dv")] +
+                [(f"{n}_{s}", C.c_int64) for n in ("q_out", "q", "k", "v", "dq", "dk", "dv") for s in ("row", "head")] +
+                [(n, C.c_void_p) for n in ("positions", "slots", "cos", "sin")] + [("table_row", C.c_int64)] +
+                [(n, C.c_int32) for n in ("positions_are_i64", "slots_are_i64", "tables_are_f32", "n_positions", "rotary_dim",
+                                          "n_tokens", "n_heads", "interleaved")] + [("status", C.c_void_p)])
+
+
+class Attention(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("out", "q", "lse")] + [(n, C.c_int64) for n in ("q_row", "q_head", "out_row", "out_head")] +
+                [(n, C.c_void_p) for n in ("table", "lens", "prefix_table", "prefix_lens", "group_starts")] +
+                [(n, C.c_int64) for n in ("table_row", "prefix_table_row")] +
+                [(n, C.c_int32) for n in ("max_pages", "max_prefix_pages", "n_requests", "n_groups", "n_heads")] +
+                [("scale", C.c_float), ("status", C.c_void_p)])
+
+
+class Int4(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("y", "x", "codes", "scales", "zeros", "add")] + [(n, C.c_int64) for n in ("x_row", "y_row", "add_row")] +
+                [(n, C.c_int32) for n in ("n_tokens", "n_in", "n_out", "group")])
+
+
 # name -> (restype, argtypes); every symbol the headers under include/ declare
 SYMBOLS = {
     "b200_lora_arch": (C.c_int, []),
@@ -88,6 +114,11 @@ SYMBOLS = {
     "b200_lora_apply_tp": (C.c_int, [C.POINTER(Proj), C.c_int32, C.POINTER(Adapters), C.c_void_p, C.c_int32,
                                      C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
                                      C.c_size_t, C.POINTER(TpContext), C.c_int32, C.c_void_p]),
+    # include/b200_decode.h
+    "b200_kv_append": (C.c_int, [C.POINTER(Append), C.POINTER(KvCache), C.c_int32, C.c_void_p]),
+    "b200_prefix_attention_workspace_bytes": (C.c_size_t, [C.c_int32] * 5),
+    "b200_prefix_attention": (C.c_int, [C.POINTER(Attention), C.POINTER(KvCache), C.c_int32, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "b200_int4_linear": (C.c_int, [C.POINTER(Int4), C.c_int32, C.c_int32, C.c_void_p]),
     # include/b200_cpu_assist.h
     "b200_xfer_register_pinned": (C.c_int, [C.c_void_p, C.c_size_t]),
     "b200_xfer_unregister_pinned": (C.c_int, [C.c_void_p]),

@@ -18,6 +18,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
 #include <string.h>
@@ -26,6 +27,7 @@
 #include <mutex>
 #include <vector>
 
+#include "b200_decode.h"
 #include "b200_lora.h"
 
 namespace {
@@ -458,6 +460,176 @@ PyObject* py_use_key(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return key.o;
 }
 
+// ---- the operators around the delta (include/b200_decode.h) ------------------------------------------
+// A tensor argument on `device` (the first one's sets it); None gives null when `optional`.
+struct Operands {
+    int device = -1;
+    bool take(PyObject* o, bool optional, const at::Tensor*& t) {
+        t = nullptr;
+        if (o == Py_None) return optional;
+        if (!THPVariable_Check(o)) return false;
+        t = &THPVariable_Unpack(o);
+        if (!t->is_cuda() || t->layout() != at::kStrided) return false;
+        if (device < 0) device = t->get_device();
+        return t->get_device() == device;
+    }
+};
+bool shaped(const at::Tensor& t, int64_t a, int64_t b, int64_t c) {
+    return t.dim() == 3 && t.size(0) == a && t.size(1) == b && t.size(2) == c && (t.stride(2) == 1 || c == 1);
+}
+bool index_type(const at::Tensor& t) { return t.scalar_type() == at::kInt || t.scalar_type() == at::kLong; }
+bool vector_of(const at::Tensor& t, int64_t n) { return t.dim() == 1 && t.size(0) == n && (t.stride(0) == 1 || n <= 1); }
+bool fits_int(int64_t n) { return n >= 0 && n <= 0x7fffffff; }
+bool int_word(const at::Tensor* t) { return !t || (t->scalar_type() == at::kInt && t->numel() == 1); }
+
+// k_cache and v_cache [pages, page, heads, dim] with the same strides
+bool read_cache(const at::Tensor& k, const at::Tensor& v, b200_kv_cache& c) {
+    if (k.dim() != 4 || v.sizes() != k.sizes() || v.strides() != k.strides() || k.scalar_type() != v.scalar_type() || k.numel() == 0) return false;
+    if (k.stride(3) != 1 && k.size(3) != 1) return false;
+    for (int i = 0; i < 4; ++i)
+        if (!fits_int(k.size(i))) return false;
+    c = b200_kv_cache{k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), (int32_t)k.size(0), (int32_t)k.size(1),
+                      (int32_t)k.size(2), (int32_t)k.size(3)};
+    return true;
+}
+
+// append_kv(q_out, q, k, v, k_cache, v_cache, positions, slots, cos, sin, dq, dk, dv, interleaved, status) -> status code
+PyObject* py_append_kv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 15) return slow();
+    Operands ops;
+    const at::Tensor* t[13];
+    for (int i = 0; i < 13; ++i)
+        if (!ops.take(args[i], i >= 10, t[i])) return slow();
+    const at::Tensor* word;
+    if (!ops.take(args[14], true, word) || !int_word(word)) return slow();
+    const int inter = PyObject_IsTrue(args[13]);
+    if (inter < 0) return slow();
+    const at::Tensor &q_out = *t[0], &q = *t[1], &k = *t[2], &v = *t[3], &pos = *t[6], &slots = *t[7], &cs = *t[8], &sn = *t[9];
+    b200_kv_cache c;
+    int io;
+    if (!read_cache(*t[4], *t[5], c) || !dtype_code(q.scalar_type(), io) || io == B200_LORA_F32 || q.dim() != 3) return slow();
+    const int64_t n = q.size(0), hq = q.size(1), d = c.head_dim, hk = c.n_kv_heads;
+    if (!fits_int(n) || !fits_int(hq) || hq < 1 || !shaped(q, n, hq, d) || !shaped(q_out, n, hq, d) || !shaped(k, n, hk, d) || !shaped(v, n, hk, d)) return slow();
+    for (int i = 0; i < 6; ++i)
+        if (t[i]->scalar_type() != q.scalar_type()) return slow();
+    b200_append a;
+    memset(&a, 0, sizeof(a));
+    for (int i = 10; i < 13; ++i)
+        if (t[i] && (t[i]->scalar_type() != q.scalar_type() || !shaped(*t[i], n, i == 10 ? hq : hk, d))) return slow();
+    if (!vector_of(pos, n) || !vector_of(slots, n) || !index_type(pos) || !index_type(slots)) return slow();
+    if (cs.dim() != 2 || sn.sizes() != cs.sizes() || sn.strides() != cs.strides() || cs.scalar_type() != sn.scalar_type() || !fits_int(cs.size(0)) || cs.size(0) < 1 ||
+        cs.size(1) < 1 || 2 * cs.size(1) > d || (cs.stride(1) != 1 && cs.size(1) != 1) || (cs.scalar_type() != at::kFloat && cs.scalar_type() != q.scalar_type()))
+        return slow();
+    a.q_out = q_out.data_ptr(); a.q = q.data_ptr(); a.k = k.data_ptr(); a.v = v.data_ptr();
+    a.q_out_row = q_out.stride(0); a.q_out_head = q_out.stride(1); a.q_row = q.stride(0); a.q_head = q.stride(1);
+    a.k_row = k.stride(0); a.k_head = k.stride(1); a.v_row = v.stride(0); a.v_head = v.stride(1);
+    if (t[10]) { a.dq = t[10]->data_ptr(); a.dq_row = t[10]->stride(0); a.dq_head = t[10]->stride(1); }
+    if (t[11]) { a.dk = t[11]->data_ptr(); a.dk_row = t[11]->stride(0); a.dk_head = t[11]->stride(1); }
+    if (t[12]) { a.dv = t[12]->data_ptr(); a.dv_row = t[12]->stride(0); a.dv_head = t[12]->stride(1); }
+    a.positions = pos.data_ptr(); a.slots = slots.data_ptr(); a.cos = cs.data_ptr(); a.sin = sn.data_ptr();
+    a.table_row = cs.stride(0);
+    a.positions_are_i64 = pos.scalar_type() == at::kLong; a.slots_are_i64 = slots.scalar_type() == at::kLong;
+    a.tables_are_f32 = cs.scalar_type() == at::kFloat;
+    a.n_positions = (int32_t)cs.size(0); a.rotary_dim = (int32_t)(2 * cs.size(1)); a.n_tokens = (int32_t)n; a.n_heads = (int32_t)hq;
+    a.interleaved = inter;
+    a.status = word ? static_cast<int32_t*>(word->data_ptr()) : nullptr;
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)ops.device);
+    void* stream = stream_of(q);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = n == 0 ? 0 : b200_kv_append(&a, &c, io, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+// prefix_attention(out, q, k_cache, v_cache, block_table, lens, prefix_table, prefix_lens, group_starts, scale, lse, status)
+// -> status code.  The workspace comes from torch's allocator for the call, so it belongs to the stream or to the
+// graph that is being captured.
+PyObject* py_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 12) return slow();
+    Operands ops;
+    const at::Tensor *t[9], *lse, *word;
+    for (int i = 0; i < 9; ++i)
+        if (!ops.take(args[i], i >= 6, t[i])) return slow();
+    if (!ops.take(args[10], true, lse) || !ops.take(args[11], true, word) || !int_word(word)) return slow();
+    const double scale = PyFloat_AsDouble(args[9]);
+    if (PyErr_Occurred()) return slow();
+    const at::Tensor &out = *t[0], &q = *t[1], &table = *t[4], &lens = *t[5];
+    b200_kv_cache c;
+    int io;
+    if (!read_cache(*t[2], *t[3], c) || !dtype_code(q.scalar_type(), io) || io == B200_LORA_F32 || q.dim() != 3) return slow();
+    const int64_t b = q.size(0), hq = q.size(1), d = c.head_dim;
+    if (!fits_int(b) || !fits_int(hq) || hq < 1 || !shaped(q, b, hq, d) || !shaped(out, b, hq, d)) return slow();
+    for (int i = 0; i < 4; ++i)
+        if (t[i]->scalar_type() != q.scalar_type()) return slow();
+    auto table_of = [](const at::Tensor& x, int64_t rows) {
+        return x.dim() == 2 && x.size(0) == rows && x.scalar_type() == at::kInt && (x.stride(1) == 1 || x.size(1) <= 1) && fits_int(x.size(1));
+    };
+    if (!table_of(table, b) || !vector_of(lens, b) || lens.scalar_type() != at::kInt) return slow();
+    b200_attention a;
+    memset(&a, 0, sizeof(a));
+    if (t[6] || t[7] || t[8]) {
+        if (!t[6] || !t[7] || !t[8]) return slow();
+        const int64_t g = t[6]->size(0);
+        if (!fits_int(g) || !table_of(*t[6], g) || !vector_of(*t[7], g) || !vector_of(*t[8], g + 1) || t[7]->scalar_type() != at::kInt ||
+            t[8]->scalar_type() != at::kInt)
+            return slow();
+        a.n_groups = (int32_t)g;
+        a.prefix_table = static_cast<const int32_t*>(t[6]->data_ptr()); a.prefix_table_row = t[6]->stride(0); a.max_prefix_pages = (int32_t)t[6]->size(1);
+        a.prefix_lens = static_cast<const int32_t*>(t[7]->data_ptr()); a.group_starts = static_cast<const int32_t*>(t[8]->data_ptr());
+    }
+    if (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != b || lse->size(1) != hq || !lse->is_contiguous())) return slow();
+    a.out = out.data_ptr(); a.q = q.data_ptr(); a.lse = lse ? static_cast<float*>(lse->data_ptr()) : nullptr;
+    a.q_row = q.stride(0); a.q_head = q.stride(1); a.out_row = out.stride(0); a.out_head = out.stride(1);
+    a.table = static_cast<const int32_t*>(table.data_ptr()); a.table_row = table.stride(0); a.max_pages = (int32_t)table.size(1);
+    a.lens = static_cast<const int32_t*>(lens.data_ptr());
+    a.n_requests = (int32_t)b; a.n_heads = (int32_t)hq; a.scale = (float)scale;
+    a.status = word ? static_cast<int32_t*>(word->data_ptr()) : nullptr;
+    if (b == 0) return PyLong_FromLong(0);
+    const size_t bytes = b200_prefix_attention_workspace_bytes((int32_t)b, a.n_groups, (int32_t)hq, c.n_kv_heads, c.head_dim);
+    if (bytes == 0) return slow();
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)ops.device);
+    void* stream = stream_of(q);
+    const at::Tensor ws = at::empty({(int64_t)bytes}, at::TensorOptions().dtype(at::kByte).device(q.device()));
+    void* ws_ptr = ws.data_ptr();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = b200_prefix_attention(&a, &c, io, ws_ptr, bytes, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
+// int4_linear(y, x, codes, scales, zeros, add) -> status code
+PyObject* py_int4_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    if (nargs != 6) return slow();
+    Operands ops;
+    const at::Tensor* t[6];
+    for (int i = 0; i < 6; ++i)
+        if (!ops.take(args[i], i >= 4, t[i])) return slow();
+    const at::Tensor &y = *t[0], &x = *t[1], &codes = *t[2], &scales = *t[3];
+    int io, yd;
+    if (!dtype_code(x.scalar_type(), io) || io == B200_LORA_F32 || !dtype_code(y.scalar_type(), yd) || (yd != io && yd != B200_LORA_F32)) return slow();
+    if (y.dim() != 2 || x.dim() != 2 || codes.dim() != 2 || scales.dim() != 2) return slow();
+    const int64_t n = x.size(0), k = x.size(1), out = codes.size(0), groups = scales.size(1);
+    if (!fits_int(n) || !fits_int(k) || !fits_int(out) || k < 1 || out < 1 || groups < 1 || k % groups != 0) return slow();
+    const int64_t group = k / groups;
+    if (group != 32 && group != 64 && group != 128) return slow();
+    if (codes.scalar_type() != at::kByte || codes.size(1) * 2 != k || !codes.is_contiguous() || scales.scalar_type() != x.scalar_type() || scales.size(0) != out ||
+        !scales.is_contiguous() || y.size(0) != n || y.size(1) != out || (x.stride(1) != 1) || (y.stride(1) != 1 && out != 1))
+        return slow();
+    if (t[4] && (t[4]->scalar_type() != at::kByte || t[4]->sizes() != scales.sizes() || !t[4]->is_contiguous())) return slow();
+    if (t[5] && (t[5]->scalar_type() != y.scalar_type() || t[5]->sizes() != y.sizes() || (t[5]->stride(1) != 1 && out != 1))) return slow();
+    const b200_int4 a{y.data_ptr(), x.data_ptr(), codes.data_ptr(), scales.data_ptr(), t[4] ? t[4]->data_ptr() : nullptr, t[5] ? t[5]->data_ptr() : nullptr,
+                      x.stride(0), y.stride(0), t[5] ? t[5]->stride(0) : 0, (int32_t)n, (int32_t)k, (int32_t)out, (int32_t)group};
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)ops.device);
+    void* stream = stream_of(x);
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = n == 0 ? 0 : b200_int4_linear(&a, io, yd, stream);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+}
+
 PyMethodDef kMethods[] = {
     {"apply", (PyCFunction)(void*)guarded<py_apply>, METH_FASTCALL, nullptr},
     {"plan_build", (PyCFunction)(void*)guarded<py_plan_build>, METH_FASTCALL, nullptr},
@@ -466,6 +638,9 @@ PyMethodDef kMethods[] = {
     {"bgmv_static", (PyCFunction)(void*)guarded<py_bgmv_static>, METH_FASTCALL, nullptr},
     {"stream_key", (PyCFunction)(void*)guarded<py_stream_key>, METH_FASTCALL, nullptr},
     {"use_key", (PyCFunction)(void*)guarded<py_use_key>, METH_FASTCALL, nullptr},
+    {"append_kv", (PyCFunction)(void*)guarded<py_append_kv>, METH_FASTCALL, nullptr},
+    {"prefix_attention", (PyCFunction)(void*)guarded<py_prefix_attention>, METH_FASTCALL, nullptr},
+    {"int4_linear", (PyCFunction)(void*)guarded<py_int4_linear>, METH_FASTCALL, nullptr},
     {"bgmv_register", py_bgmv_register, METH_VARARGS, nullptr},
     {"bgmv_forget", (PyCFunction)(void*)guarded<py_bgmv_forget>, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -12,12 +12,14 @@ namespace {
 
 thread_local char g_last_error[256] = "";
 
-int cuda_fail(cudaError_t e) {
+}  // namespace
+
+int b200lora::cuda_fail(cudaError_t e) {
     strncpy(g_last_error, cudaGetErrorString(e), sizeof(g_last_error) - 1);
     return B200_LORA_ERR_CUDA;
 }
 
-int sm_count() {
+int b200lora::sm_count() {
     static int cached[64] = {0};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
@@ -28,6 +30,8 @@ int sm_count() {
     }
     return cached[dev];
 }
+
+namespace {
 
 // ---- tensor maps for the TMA kernels --------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

@@ -302,6 +302,10 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
+// ---- shared by the entry points (lora_api.cu) ------------------------------------------------
+int cuda_fail(cudaError_t e);             // keeps the error's text for b200_lora_last_cuda_error; returns B200_LORA_ERR_CUDA
+int sm_count();                           // of the current device
+
 // ---- launchers implemented by the kernel files ---------------------------------------------
 struct PlanAdapters {          // what the plan bakes into its unit records
     const int* ranks;
