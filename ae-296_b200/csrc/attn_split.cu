@@ -9,8 +9,9 @@
 // its neighbours up, and multiplies with mma.sync: decode reads every key for at most 16 query rows, some 16
 // products a byte, so the copies bound it and not the multiplications.  The weights 2^(z - m) go into the second
 // product as two 16-bit numbers (the value rounded, and what the rounding dropped), so nothing is lost against fp32.
-#include "decode_common.cuh"
-#include "lora_pipe.cuh"
+#include <type_traits>
+
+#include "attn_common.cuh"
 
 namespace b200lora {
 
@@ -27,11 +28,6 @@ template <int D> struct Ring {
     static constexpr int kBytes = kWarps * kStages * kStage;
 };
 
-__device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ldsm4(unsigned addr, unsigned (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -41,38 +37,16 @@ __device__ __forceinline__ void ldsm4t(unsigned addr, unsigned (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-struct Entity { int rows, tiles, chunks, keys, first; };     // first: request of the first row
-
-__device__ __forceinline__ int clamped_keys(const AttnParams& p, int n, int pages, int& bad) {
-    const int most = pages << p.page_shift;                   // fits: checked on the host
-    if (n < 0 || n > most) bad |= B200_DECODE_BAD_LENGTH;
-    return n < 0 ? 0 : n > most ? most : n;
-}
-// Entity e: group e, or request e - n_groups.  `groups` false: the group starts cannot be used, groups have no rows.
-__device__ __forceinline__ Entity entity_of(const AttnParams& p, int e, bool groups, int& bad) {
+// Entity e of this kernel: group e, or request e - n_groups
+__device__ __forceinline__ Entity entity_of(const AttnParams& p, int e, bool usable, int& bad) {
+    if (e < p.a.n_groups) return group_of<kAttnRows, kKeys, false>(p, e, usable, bad);
     Entity t;
-    const int g = p.a.n_groups;
-    if (e < g) {
-        const int s0 = p.a.group_starts[e], s1 = p.a.group_starts[e + 1];
-        const bool fine = s0 >= 0 && s1 >= s0 && s1 <= p.a.n_requests;
-        if (!fine) bad |= B200_DECODE_BAD_GROUPS;
-        t.first = s0;
-        t.rows = fine && groups ? (s1 - s0) * p.per : 0;
-        t.tiles = (t.rows + kAttnRows - 1) / kAttnRows;
-        t.keys = t.rows ? clamped_keys(p, p.a.prefix_lens[e], p.a.max_prefix_pages, bad) : 0;
-    } else {
-        t.first = e - g;
-        t.rows = p.per;
-        t.tiles = p.req_tiles;
-        t.keys = clamped_keys(p, p.a.lens[e - g], p.a.max_pages, bad);
-    }
+    t.first = e - p.a.n_groups;
+    t.rows = p.per;
+    t.tiles = p.req_tiles;
+    t.keys = clamped_keys(p, p.a.lens[t.first], p.a.max_pages, bad);
     t.chunks = (t.keys + kKeys - 1) / kKeys;
     return t;
-}
-
-__device__ __forceinline__ long long unit_of_worker(long long total, int w, int workers) { return total * w / workers; }
-__device__ __forceinline__ int worker_of_unit(long long total, long long u, int workers) {
-    return (int)(((u + 1) * workers - 1) / total);
 }
 
 template <int D>
@@ -101,48 +75,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
     __shared__ int key_mask[kWarps][R::kStages];
     __shared__ int bad_all;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_wait_prior();
-    if (tid == 0) { pdl_launch_dependents(); bad_all = 0; }
-    __syncthreads();
-
-    // ---- units before each entity, tiles before each group; written out once for the join
-    const int n_ent = p.a.n_groups + p.a.n_requests;
-    bool groups = p.a.n_groups > 0;
-    for (int attempt = 0; attempt < 2; ++attempt) {
-        unsigned long long carry = 0;
-        int bad = 0;
-        for (int base = 0; base < n_ent; base += kThreads) {
-            const int e = base + tid;
-            unsigned long long v = 0;
-            if (e < n_ent) {
-                const Entity t = entity_of(p, e, groups, bad);
-                v = ((unsigned long long)(e < p.a.n_groups ? t.tiles : 0) << 32) | (unsigned)(t.tiles * t.chunks);
-            }
-            unsigned long long inc = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const unsigned long long up = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += up;
-            }
-            if (lane == 31) warp_sum[warp] = inc;
-            __syncthreads();
-            unsigned long long before = carry, all = 0;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) { if (w < warp) before += warp_sum[w]; all += warp_sum[w]; }
-            if (e < n_ent) {
-                su[e] = (int)(unsigned)(before + inc - v);
-                if (e < p.a.n_groups) st[e] = (int)((before + inc - v) >> 32);
-            }
-            carry += all;
-            __syncthreads();
-        }
-        if (tid == 0) { su[n_ent] = (int)(unsigned)carry; st[p.a.n_groups] = (int)(carry >> 32); }
-        if (bad) atomicOr(&bad_all, bad);
-        __syncthreads();
-        // starts that descend somewhere: no group has a prefix
-        if (!groups || !(bad_all & B200_DECODE_BAD_GROUPS)) break;
-        groups = false;
+    // Behind the wide kernel, which leaves alone what this one reads, only its end is waited for (at this one's own):
+    // whatever came before the wide kernel is complete when a block of this one runs.
+    if (!p.wide_tiles) {
+        pdl_wait_prior();
+        if (tid == 0) pdl_launch_dependents();
     }
+    if (tid == 0) bad_all = 0;
+    __syncthreads();
+    // units before each entity, row tiles before each group; written out once for the join
+    const int n_ent = p.a.n_groups + p.a.n_requests;
+    const bool groups = scan_units<kThreads>(n_ent, p.a.n_groups, su, st, warp_sum, &bad_all, [&](int e, bool usable, int& bad) {
+        const Entity t = entity_of(p, e, usable, bad);
+        return ((unsigned long long)(e < p.a.n_groups ? t.tiles : 0) << 32) | (unsigned)(t.tiles * t.chunks);
+    });
     if (blockIdx.x == 0) {
         for (int i = tid; i <= n_ent; i += kThreads) p.units[i] = su[i];
         for (int i = tid; i <= p.a.n_groups; i += kThreads) p.tiles[i] = groups ? st[i] : -1;
@@ -153,7 +99,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
     const long long total = (long long)su[n_ent] * n_kv;
     const int workers = (int)min((long long)p.workers, total);
     const int worker = warp * gridDim.x + blockIdx.x;        // neighbours in the work on different SMs
-    if (worker >= workers) return;
+    if (worker >= workers) {
+        pdl_wait_prior();
+        pdl_launch_dependents();
+        return;
+    }
     long long u = unit_of_worker(total, worker, workers);
     const long long u_end = unit_of_worker(total, worker + 1, workers);
     const unsigned ring = smem_u32(smem) + warp * R::kStages * R::kStage;
@@ -163,12 +113,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
     while (u < u_end) {
         // ---- the item of unit u
         const int uh = (int)(u / n_kv);
-        int lo = 0, hi = n_ent;                               // last entity with su[e] <= uh
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (su[mid] <= uh) lo = mid; else hi = mid;
-        }
-        const int e = lo;
+        const int e = entity_at(su, n_ent, uh);
         const Entity t = entity_of(p, e, groups, ignored);
         long long r = u - (long long)n_kv * su[e];
         const int per_head = t.tiles * t.chunks;
@@ -319,6 +264,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
         __syncwarp();
         u += n;
     }
+    pdl_wait_prior();
+    pdl_launch_dependents();
 }
 
 // One warp per query row: the row's parts of its group's item and of its own item, weighted by 2^(m_i - max m).
@@ -360,6 +307,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
 #pragma unroll 4
             for (int j = 0; j < n; ++j) {
                 const float wj = __shfl_sync(0xffffffffu, w, j);
+                if (wj == 0.f) continue;                       // a part without keys may have no sums either
                 const float* src = p.part + (slot + (size_t)(base + j) * pitch) * D + lane * V;
                 if constexpr (V == 4) {
                     const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
@@ -378,14 +326,25 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
             if (p.a.group_starts[mid] <= b) lo = mid; else hi = mid;
         }
         if (lo >= 0 && b < p.a.group_starts[lo + 1]) {
-            const int r = (b - p.a.group_starts[lo]) * p.per + i, tile = r / kAttnRows;
-            const int tiles = p.tiles[lo + 1] - p.tiles[lo], all = p.units[lo + 1] - p.units[lo];
+            const int r = (b - p.a.group_starts[lo]) * p.per + i, n_rows = (p.a.group_starts[lo + 1] - p.a.group_starts[lo]) * p.per;
+            const bool wide = n_rows > kAttnRows;
+            const int* units = wide ? p.wide_units : p.units;
+            const int* before = wide ? p.wide_tile : p.tiles;
+            const int tiles = before[lo + 1] - before[lo], all = units[lo + 1] - units[lo], tile = r / (wide ? kWideRows : kAttnRows);
             if (all > 0) {
                 const int chunks = all / tiles;
-                const long long u0 = (long long)n_kv * p.units[lo] + (long long)h * all + (long long)tile * chunks;
-                const size_t item = (size_t)n_kv * p.tiles[lo] + (size_t)h * tiles + tile;
-                add(item * kAttnRows + (r - tile * kAttnRows), kAttnRows, worker_of_unit(total, u0, workers),
-                    worker_of_unit(total, u0 + chunks - 1, workers));
+                const long long u0 = (long long)n_kv * units[lo] + (long long)h * all + (long long)tile * chunks;
+                const size_t item = (size_t)n_kv * before[lo] + (size_t)h * tiles + tile;
+                const long long sum = wide ? (long long)p.wide_units[n_g] * n_kv : total;
+                const int w = wide ? (int)min((long long)p.wide_workers, sum) : workers;
+                const int w0 = worker_of_unit(sum, u0, w), w1 = worker_of_unit(sum, u0 + chunks - 1, w);
+                if (!wide) add(item * kAttnRows + (r - tile * kAttnRows), kAttnRows, w0, w1);
+                else {
+                    const size_t row = attn_group_rows(p) + attn_request_rows(p) + item * kWideRows + (r - tile * kWideRows);
+                    add(row, kWideRows, w0, w1);
+                    // a tile of one stream's rows: the second stream's parts, over the other keys, lie behind them
+                    if (n_rows - tile * kWideRows <= kWideRows / 2) add(row + kWideRows / 2, kWideRows, w0, w1);
+                }
             }
         }
     }
@@ -413,8 +372,14 @@ cudaError_t launch_typed(const AttnParams& p0, int n_sm, cudaStream_t s) {
     AttnParams p = p0;
     const int grid = n_sm < kAttnMaxWorkers / kWarps ? n_sm : kAttnMaxWorkers / kWarps;
     p.workers = grid * kWarps;
+    p.wide_workers = n_sm < kWideMaxWorkers ? n_sm : kWideMaxWorkers;
     const size_t smem = Ring<D>::kBytes + 4 * ((size_t)2 * p.a.n_groups + p.a.n_requests + 2);
-    cudaError_t e = cudaFuncSetAttribute(attn_split_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    cudaError_t e = cudaSuccess;
+    if (p.wide_tiles) {
+        e = launch_attention_wide(p, std::is_same_v<T, __half> ? B200_LORA_F16 : B200_LORA_BF16, s);
+        if (e != cudaSuccess) return e;
+    }
+    e = cudaFuncSetAttribute(attn_split_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     e = launch_pdl(attn_split_kernel<T, D>, grid, kThreads, smem, s, p);
     if (e != cudaSuccess) return e;

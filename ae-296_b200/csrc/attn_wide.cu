@@ -1,0 +1,477 @@
+// The shared prefixes of larger groups: attention of up to 256 query rows (requests of the group times the query heads
+// of a cache head) against a range of the prefix's keys, on the tcgen05 tensor cores.
+//
+// With r rows a key and its value (4 D bytes) are used for 4 D r operations: above 258 rows the multiplications bound
+// the work on this GPU, and already at 32 rows the split kernel's reading of the keys once per 16 rows would.
+//
+// A block of kKeys = 128 keys is a unit.  Two streams of 128 rows each go through the units of an item:
+//     S[128, 128] = Q K^T            tcgen05.mma, Q and K from shared memory
+//     P = 2^(scale S - m)            by the stream's four warps, a thread per row, S from and P (16 bits) to TMEM
+//     O[128, D] += P V               tcgen05.mma, P from TMEM, V from shared memory (its rows are the contraction)
+// While the warps of one stream compute exponentials, the tensor core multiplies for the other.  Where an item has more
+// than 128 rows the streams hold different rows and share each block; else they hold the same rows and take the blocks in
+// turns, and each leaves a part of its own.
+//
+// The running maximum is not followed exactly: the sums are only rescaled when a row's maximum has grown by more than
+// 2^8, since fp32 sums and 16-bit weights up to 256 lose nothing by a common factor.  P is rounded to the 16-bit type
+// (relative 2^-9 or 2^-12, as often up as down): what the output's own rounding does again.
+//
+// Warps 0..3 and 4..7: the streams.  Warp 8: one thread issues the multiplications.  Warps 9..11 bring keys and values
+// into a ring of blocks by asynchronous 16-byte copies in the 128-byte swizzled layout the multiplications read, page
+// by page, whatever the page size, with zeros in place of keys behind the prefix or in pages that do not exist.
+// Every wait is bounded: on expiry the block's error word is set, control flow stays as it is and the kernel ends.
+#include <type_traits>
+
+#include "attn_common.cuh"
+
+namespace b200lora {
+
+namespace {
+
+constexpr int kStreamRows = 128;
+constexpr int kThreads = 384;
+constexpr int kCopyWarps = 3;
+constexpr int kCopyThreads = kCopyWarps * 32;
+constexpr int kTmemCols = 512;
+constexpr float kSlack = 8.f;                     // in powers of two
+
+template <int D, int RING> struct Wide {
+    static constexpr int kQ = kStreamRows * D * 2;           // a stream's queries
+    static constexpr int kBlock = kWideKeys * D * 2;         // keys or values of a unit
+    static constexpr int kBytes = 2 * kQ + RING * kBlock;
+};
+constexpr int kMaxRing = 8;
+constexpr int kMissing = 16;                      // more blocks of keys than can lie between their copies and their use
+struct WideShared {
+    uint4 missing[kMissing][kCopyWarps];          // keys of a block in pages that do not exist, as each copy warp saw them
+    unsigned long long full[kMaxRing], empty[kMaxRing], q_ready[2], s_full[2], p_ready[2], o_full[2];
+    unsigned long long warp_sum[kThreads / 32];
+    unsigned tmem, err;
+    int bad, pad;
+};
+static_assert(sizeof(WideShared) % 16 == 0, "the scan's arrays follow");
+constexpr int kSmemLimit = 232448;                // of a block
+
+__device__ __forceinline__ void tmem_alloc(unsigned smem_dst) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "n"(kTmemCols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(unsigned taddr) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "n"(kTmemCols) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(unsigned bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// D = A B^T, A and B from shared memory
+__device__ __forceinline__ void mma_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+// D += A B, A from TMEM
+__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tc_ld32(unsigned taddr, unsigned (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tc_st32(unsigned taddr, const unsigned (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+        "%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+          "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+          "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Shared-memory operands with 128-byte swizzle: panels of 64 elements, [rows][128 bytes], 16-byte piece c of row r at
+// c ^ (r % 8).  Rows are rows of the operand (K-major) or the contraction (MN-major: `panel` bytes from one 64 to the next).
+__device__ __forceinline__ unsigned long long desc_k(unsigned saddr) {
+    return (unsigned long long)((saddr >> 4) & 0x3fffu) | (1ull << 16) | ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ unsigned long long desc_mn(unsigned saddr, unsigned panel) {
+    return (unsigned long long)((saddr >> 4) & 0x3fffu) | ((unsigned long long)(panel >> 4) << 16) | ((unsigned long long)(1024 >> 4) << 32) |
+           (1ull << 46) | (2ull << 61);
+}
+// kind::f16, fp32 sums, M = 128; b_mn: the second operand's rows are the contraction
+__device__ __forceinline__ unsigned idesc_of(bool bf16, int n, bool b_mn) {
+    const unsigned fmt = bf16 ? 1u : 0u;
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | (b_mn ? 1u << 16 : 0u) | ((unsigned)(n >> 3) << 17) | ((unsigned)(kStreamRows >> 4) << 24);
+}
+// byte address of 16-byte piece `piece` of row `row` in an operand of 128 rows
+__device__ __forceinline__ unsigned swizzled(unsigned base, int row, int piece) {
+    return base + (piece >> 3) * (128 * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+}
+
+// An item's part of a worker: blocks [b0, b0 + n) of tile `tile` of cache head `h` of group `g`.
+struct Part {
+    int g, h, tile, b0, n, rows, first, keys;
+    bool dual;             // the streams hold different rows
+    size_t slot;           // first row of the part's partial results
+};
+
+__device__ __forceinline__ Part part_of(const AttnParams& p, const int* su, const int* st, bool usable, long long u, long long u_end) {
+    Part t;
+    int ignored = 0;
+    const int n_kv = p.c.n_kv_heads;
+    const int uh = (int)(u / n_kv);
+    t.g = entity_at(su, p.a.n_groups, uh);
+    const Entity e = group_of<kWideRows, kWideKeys, true>(p, t.g, usable, ignored);
+    const int per_head = e.tiles * e.chunks;
+    const long long of_entity = u - (long long)n_kv * su[t.g];
+    t.h = (int)(of_entity / per_head);
+    const int rest = (int)(of_entity - (long long)t.h * per_head);
+    t.tile = rest / e.chunks;
+    t.b0 = rest - t.tile * e.chunks;
+    t.n = (int)min((long long)(e.chunks - t.b0), u_end - u);
+    t.rows = min(kWideRows, e.rows - t.tile * kWideRows);
+    t.first = e.first;
+    t.keys = e.keys;
+    t.dual = t.rows > kStreamRows;
+    t.slot = attn_group_rows(p) + attn_request_rows(p) + ((size_t)n_kv * st[t.g] + (size_t)t.h * e.tiles + t.tile + blockIdx.x) * kWideRows;
+    return t;
+}
+
+template <typename T, int D, int RING>
+__global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_constant__ AttnParams p) {
+    extern __shared__ unsigned char smem_raw[];
+    using W = Wide<D, RING>;
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    WideShared& sh = *reinterpret_cast<WideShared*>(smem + W::kBytes);
+    int* su = reinterpret_cast<int*>(&sh + 1);
+    int* st = su + p.a.n_groups + 1;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto bar = [](unsigned long long& b) { return smem_u32(&b); };
+    unsigned* err = &sh.err;
+
+    pdl_wait_prior();
+    if (tid == 0) {
+        pdl_launch_dependents();
+        for (int i = 0; i < RING; ++i) { mbar_init(bar(sh.full[i]), kCopyThreads); mbar_init(bar(sh.empty[i]), 1); }
+        for (int s = 0; s < 2; ++s) {
+            mbar_init(bar(sh.q_ready[s]), kStreamRows);
+            mbar_init(bar(sh.p_ready[s]), kStreamRows);
+            mbar_init(bar(sh.s_full[s]), 1);
+            mbar_init(bar(sh.o_full[s]), 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        sh.err = 0u;
+        sh.bad = 0;
+    }
+    __syncthreads();
+    const int n_g = p.a.n_groups, n_kv = p.c.n_kv_heads;
+    const bool usable = scan_units<kThreads>(n_g, n_g, su, st, sh.warp_sum, &sh.bad, [&](int e, bool ok, int& bad) {
+        const Entity t = group_of<kWideRows, kWideKeys, true>(p, e, ok, bad);
+        return ((unsigned long long)t.tiles << 32) | (unsigned)(t.tiles * t.chunks);
+    });
+    if (blockIdx.x == 0)
+        for (int i = tid; i <= n_g; i += kThreads) { p.wide_units[i] = su[i]; p.wide_tile[i] = st[i]; }
+    const long long total = (long long)su[n_g] * n_kv;
+    const int workers = (int)min((long long)p.wide_workers, total);
+    if ((int)blockIdx.x >= workers) return;
+    const long long u_first = unit_of_worker(total, blockIdx.x, workers), u_end = unit_of_worker(total, blockIdx.x + 1, workers);
+    auto part_at = [&](long long u) { return part_of(p, su, st, usable, u, u_end); };
+
+    if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&sh.tmem);
+    const unsigned ring = smem_u32(smem) + 2 * W::kQ;
+    // The ring's order within a part: where the streams share blocks, K0 V0 K1 V1 ...; where they take them in turns,
+    // K0 K1 V0 K2 V1 K3 ...: what the multiplications wait for next always comes next.
+    auto k_at = [](const Part& t, int b) { return t.dual ? 2 * b : b < 2 ? b : 2 * b - 1; };
+    auto v_at = [](const Part& t, int b) { return t.dual ? 2 * b + 1 : min(2, t.n) + b + min(b, max(t.n - 2, 0)); };
+
+    if (warp >= 9) {
+        // ================= copies =================
+        const int cw = warp - 9;
+        constexpr int kPieces = D / 8, kRowsAt = 32 / kPieces;
+        const int piece = lane % kPieces, sub = lane / kPieces;
+        const int in_page = (1 << p.page_shift) - 1;
+        unsigned n = 0, n_keys = 0;              // blocks, and blocks of keys, so far
+        int pending = -1;                        // slot whose copies are in flight
+        auto arrived = [&]() {
+            if (pending < 0) return;
+            fence_async_proxy();                 // the copies wrote through the generic proxy
+            mbar_arrive(bar(sh.full[pending]));
+            pending = -1;
+        };
+        for (long long u = u_first; u < u_end;) {
+            const Part t = part_at(u);
+            const int* table = p.a.prefix_table + (long long)t.g * p.a.prefix_table_row;
+            for (int i = 0; i < 2 * t.n; ++i, ++n) {
+                bool is_v;
+                int b;
+                if (t.dual) { is_v = i & 1; b = i >> 1; }
+                else {
+                    const int lead = min(2, t.n), j = i - lead, pairs = max(t.n - 2, 0);
+                    if (j < 0) { is_v = false; b = i; }
+                    else if (j < 2 * pairs) { is_v = !(j & 1); b = is_v ? j >> 1 : (j >> 1) + 2; }
+                    else { is_v = true; b = j - pairs; }
+                }
+                const int slot = n % RING;
+                const unsigned phase = ((n / RING) & 1) ^ 1;
+                if (!mbar_try_wait(bar(sh.empty[slot]), phase)) {       // what has arrived meanwhile must not wait for this
+                    cp_wait<0>();
+                    arrived();
+                    mbar_wait(bar(sh.empty[slot]), phase, err, 1);
+                }
+                __syncwarp();
+                const unsigned dst = ring + slot * W::kBlock;
+                const int key0 = (t.b0 + b) * kWideKeys;
+                const T* base = static_cast<const T*>(is_v ? p.c.v : p.c.k) + (long long)t.h * p.c.head_stride + piece * 8;
+                uint4 missing = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 4
+                for (int g = cw; g < kWideKeys / kRowsAt; g += kCopyWarps) {
+                    const int row = g * kRowsAt + sub, key = key0 + row;
+                    const bool wanted = key < t.keys;
+                    const int page = wanted ? __ldg(table + (key >> p.page_shift)) : 0;
+                    const bool fine = wanted && (unsigned)page < (unsigned)p.c.n_pages;
+                    const long long at = fine ? (long long)page * p.c.page_stride + (long long)(key & in_page) * p.c.token_stride : 0;
+                    cp_async16(swizzled(dst, row, piece), base + at, fine);
+                    const unsigned lost = __ballot_sync(0xffffffffu, wanted && !fine && piece == 0);
+                    if (lost) {
+                        if (lane == 0 && p.a.status) atomicOr(p.a.status, B200_DECODE_BAD_PAGE);
+                        unsigned rows = 0;
+#pragma unroll
+                        for (int k = 0; k < kRowsAt; ++k) rows |= ((lost >> (k * kPieces)) & 1u) << ((g * kRowsAt + k) & 31);
+                        const int word = (g * kRowsAt) >> 5;
+                        missing.x |= word == 0 ? rows : 0u; missing.y |= word == 1 ? rows : 0u;
+                        missing.z |= word == 2 ? rows : 0u; missing.w |= word == 3 ? rows : 0u;
+                    }
+                }
+                cp_commit();
+                if (!is_v) {
+                    if (lane == 0) sh.missing[n_keys % kMissing][cw] = missing;
+                    ++n_keys;
+                }
+                if (pending >= 0) { cp_wait<1>(); arrived(); }
+                pending = slot;
+            }
+            u += t.n;
+        }
+        cp_wait<0>();
+        arrived();
+    } else if (warp == 8) {
+        // ================= multiplications =================
+        const bool bf16 = Cvt<T>::is_bf16;
+        const unsigned id_s = idesc_of(bf16, kWideKeys, false), id_o = idesc_of(bf16, D, true);
+        unsigned n = 0, parts[2] = {0u, 0u}, rounds[2] = {0u, 0u};       // blocks, each stream's parts and rounds so far
+        for (long long u = u_first; u < u_end;) {
+            const Part t = part_at(u);
+            auto block_of = [&](int s, int r) { return t.dual ? r : 2 * r + s; };
+            auto wait_full = [&](int at) { const unsigned k = n + at; mbar_wait(bar(sh.full[k % RING]), (k / RING) & 1, err, 2); tc_fence_after(); };
+            auto scores = [&](int s, int b) {
+                const int at = k_at(t, b);
+                wait_full(at);
+                if (lane == 0) {
+                    const unsigned slot = (n + at) % RING, ka = ring + slot * W::kBlock, qa = smem_u32(smem) + s * W::kQ;
+#pragma unroll
+                    for (int k = 0; k < D / 16; ++k) {
+                        const unsigned off = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                        mma_ss(tmem + s * 128, desc_k(qa + off), desc_k(ka + off), id_s, k != 0);
+                    }
+                    tc_commit(bar(sh.s_full[s]));
+                    if (!t.dual || s == 1) tc_commit(bar(sh.empty[slot]));
+                }
+                __syncwarp();
+            };
+            for (int s = 0; s < 2; ++s)
+                if (block_of(s, 0) < t.n) {                      // a stream without a block has no queries either
+                    mbar_wait(bar(sh.q_ready[s]), parts[s] & 1, err, 3);
+                    ++parts[s];
+                    tc_fence_after();
+                    scores(s, block_of(s, 0));
+                }
+            for (int r = 0; block_of(0, r) < t.n; ++r)
+                for (int s = 0; s < 2; ++s) {
+                    const int b = block_of(s, r);
+                    if (b >= t.n) continue;
+                    mbar_wait(bar(sh.p_ready[s]), rounds[s] & 1, err, 4);
+                    ++rounds[s];
+                    const int at = v_at(t, b);
+                    wait_full(at);
+                    if (lane == 0) {
+                        const unsigned slot = (n + at) % RING, va = ring + slot * W::kBlock;
+#pragma unroll
+                        for (int k = 0; k < kWideKeys / 16; ++k)
+                            mma_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, desc_mn(va + k * 2048, 128 * 128), id_o, (r | k) != 0);
+                        if (!t.dual || s == 1) tc_commit(bar(sh.empty[slot]));
+                        if (block_of(s, r + 1) >= t.n) tc_commit(bar(sh.o_full[s]));
+                    }
+                    __syncwarp();
+                    if (block_of(s, r + 1) < t.n) scores(s, block_of(s, r + 1));
+                }
+            n += 2 * t.n;
+            u += t.n;
+        }
+    } else {
+        // ================= the streams =================
+        const int s = warp >> 2, row = tid & 127;
+        const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
+        const unsigned s_tm = tmem + lanes + s * 128, o_tm = tmem + lanes + 256 + s * 128;
+        // scores are compared as they come from the multiplication: a negative scale goes into the queries' signs
+        const unsigned flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
+        const float scale = fabsf(p.scale_log2);
+        const float kLift = std::is_same_v<T, __half> ? 7.f : 0.f;     // fp16 weights up to 2^(8 + 7), far from its smallest numbers
+        unsigned rounds = 0, outs = 0, n_keys = 0;
+        for (long long u = u_first; u < u_end;) {
+            const Part t = part_at(u);
+            const int r_in = t.dual ? s * kStreamRows + row : row;
+            const bool live = r_in < t.rows;
+            const int step = t.dual ? 1 : 2, b_first = t.dual ? 0 : s;
+            // ---- queries to shared memory (the stream's last multiplication that reads them is complete)
+            if (b_first < t.n) {
+                const int ra = t.tile * kWideRows + (live ? r_in : 0);
+                const T* q = static_cast<const T*>(p.a.q) + (long long)(t.first + ra / p.per) * p.a.q_row + (long long)(t.h * p.per + ra % p.per) * p.a.q_head;
+                const unsigned qa = smem_u32(smem) + s * W::kQ;
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    uint4 v = *reinterpret_cast<const uint4*>(q + c * 8);
+                    if (!live) v = make_uint4(0u, 0u, 0u, 0u);
+                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};"
+                                 ::"r"(swizzled(qa, row, c)), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
+                }
+                fence_async_proxy();
+                mbar_arrive(bar(sh.q_ready[s]));
+            }
+            const bool warp_live = __ballot_sync(0xffffffffu, live) != 0u;
+            float m = -INFINITY, l = 0.f;                        // sums are relative to 2^(m - kLift)
+            for (int b = b_first; b < t.n; b += step, ++rounds) {
+                mbar_wait(bar(sh.s_full[s]), rounds & 1, err, 5);
+                tc_fence_after();
+                if (warp_live) {
+                    unsigned zr[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tc_ld32(s_tm + c * 32, zr[c]);
+                    auto z = [&](int j) { return __uint_as_float(zr[j >> 5][j & 31]); };
+                    tc_wait_ld();
+                    // keys behind the prefix, or in pages that do not exist
+                    const uint4* lost = sh.missing[(n_keys + b) % kMissing];
+                    const uint4 w0 = lost[0], w1 = lost[1], w2 = lost[2];
+                    const int valid = t.keys - (t.b0 + b) * kWideKeys;
+                    if (valid < kWideKeys || ((w0.x | w1.x | w2.x) | (w0.y | w1.y | w2.y) | (w0.z | w1.z | w2.z) | (w0.w | w1.w | w2.w))) {
+                        const unsigned gone[4] = {w0.x | w1.x | w2.x, w0.y | w1.y | w2.y, w0.z | w1.z | w2.z, w0.w | w1.w | w2.w};
+#pragma unroll
+                        for (int j = 0; j < 128; ++j)
+                            if (j >= valid || (gone[j >> 5] >> (j & 31) & 1u)) zr[j >> 5][j & 31] = 0xff800000u;      // -infinity
+                    }
+                    float x[4] = {z(0), z(1), z(2), z(3)};
+#pragma unroll
+                    for (int j = 4; j < 128; ++j) x[j & 3] = fmaxf(x[j & 3], z(j));
+                    const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * scale;
+                    if (b == b_first) m = top;
+                    else {
+                        const bool grown = top > m + kSlack || (m == -INFINITY && top > m);
+                        if (__any_sync(0xffffffffu, grown)) {
+                            const float f = grown ? (m == -INFINITY ? 0.f : ex2(m - top)) : 1.f;
+                            if (grown) m = top;
+                            l *= f;
+#pragma unroll
+                            for (int c = 0; c < D / 32; ++c) {
+                                unsigned o[32];
+                                tc_ld32(o_tm + c * 32, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                                tc_st32(o_tm + c * 32, o);
+                            }
+                            tc_wait_st();
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m - kLift;      // nothing yet: every weight is 0
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        unsigned w[32];
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float a = ex2(fmaf(z(c * 64 + 2 * j), scale, -ref)), d = ex2(fmaf(z(c * 64 + 2 * j + 1), scale, -ref));
+                            sum[(2 * j) & 3] += a;
+                            sum[(2 * j + 1) & 3] += d;
+                            w[j] = Cvt<T>::pack2(a, d);
+                        }
+                        tc_st32(s_tm + c * 32, w);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tc_wait_st();
+                }
+                tc_fence_before();
+                mbar_arrive(bar(sh.p_ready[s]));
+            }
+            // ---- this worker's part of the rows
+            const size_t out_row = t.slot + s * kStreamRows + row;
+            if (b_first < t.n) {
+                mbar_wait(bar(sh.o_full[s]), outs & 1, err, 6);
+                ++outs;
+                tc_fence_after();
+                if (warp_live) {
+                    float* dst = p.part + out_row * D;
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        unsigned o[32];
+                        tc_ld32(o_tm + c * 32, o);
+                        tc_wait_ld();
+                        if (live) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                reinterpret_cast<uint4*>(dst + c * 32)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                        }
+                    }
+                    tc_fence_before();
+                }
+                if (live) p.part_ml[out_row] = make_float2(m == -INFINITY ? m : m - kLift, l);
+            } else if (live) p.part_ml[out_row] = make_float2(-INFINITY, 0.f);
+            n_keys += t.n;
+            u += t.n;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 8) tmem_dealloc(tmem);
+    if (tid == 0 && sh.err && p.a.status) atomicOr(p.a.status, B200_DECODE_TIMEOUT);
+}
+
+template <typename T, int D, int RING>
+cudaError_t launch_ring(const AttnParams& p, size_t scan, cudaStream_t s) {
+    const size_t smem = Wide<D, RING>::kBytes + sizeof(WideShared) + scan + 1024;
+    const cudaError_t e = cudaFuncSetAttribute(attn_wide_kernel<T, D, RING>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(attn_wide_kernel<T, D, RING>, p.wide_workers, kThreads, smem, s, p);
+}
+template <typename T>
+cudaError_t launch_typed(const AttnParams& p, cudaStream_t s) {
+    const size_t scan = 8 * ((size_t)p.a.n_groups + 1);
+    if (p.c.head_dim == 64) return launch_ring<T, 64, 8>(p, scan, s);
+    // as many blocks as fit beside the scan's arrays
+    if (Wide<128, 5>::kBytes + sizeof(WideShared) + scan + 1024 <= kSmemLimit) return launch_ring<T, 128, 5>(p, scan, s);
+    return launch_ring<T, 128, 4>(p, scan, s);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_wide(const AttnParams& p, int dtype, cudaStream_t s) {
+    return dtype == B200_LORA_F16 ? launch_typed<__half>(p, s) : launch_typed<__nv_bfloat16>(p, s);
+}
+
+}  // namespace b200lora

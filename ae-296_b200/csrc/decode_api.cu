@@ -1,4 +1,6 @@
 // extern "C" entry points declared in include/b200_decode.h: argument checks and launches only.
+#include <cfloat>
+
 #include "decode_common.cuh"
 
 using namespace b200lora;
@@ -24,12 +26,18 @@ int attention_sizes(AttnParams& p) {
     p.per = p.a.n_heads / p.c.n_kv_heads;
     p.req_tiles = (p.per + kAttnRows - 1) / kAttnRows;
     p.req_rows = p.per < kAttnRows ? p.per : kAttnRows;
-    p.max_group_tiles = p.a.n_groups == 0 ? 0 : (int)(((int64_t)p.a.n_requests * p.per + kAttnRows - 1) / kAttnRows) + p.a.n_groups;
+    const int rows = p.a.n_requests * p.per;                  // at most 4096 * 1024
+    const bool wide = p.a.n_groups > 0 && rows > kAttnRows;
+    // groups of at most kAttnRows rows, and wide ones (of which there are fewer than rows / kAttnRows)
+    p.max_group_tiles = p.a.n_groups;
+    const int wide_groups = rows / (kAttnRows + 1);
+    p.wide_tiles = wide ? (rows + kWideRows - 1) / kWideRows + (p.a.n_groups < wide_groups ? p.a.n_groups : wide_groups) : 0;
     return B200_LORA_OK;
 }
 
 size_t attention_bytes(const AttnParams& p) {
-    return attn_rows(p) * ((size_t)p.c.head_dim * 4 + 8) + 4 * ((size_t)2 * p.a.n_groups + p.a.n_requests + 2) + 64;
+    return (attn_group_rows(p) + attn_request_rows(p) + attn_wide_rows(p)) * ((size_t)p.c.head_dim * 4 + 8) +
+           4 * ((size_t)4 * p.a.n_groups + p.a.n_requests + 4) + 64;
 }
 
 }  // namespace
@@ -79,7 +87,9 @@ extern "C" int b200_prefix_attention(const b200_attention* a, const b200_kv_cach
     // keys of a row of a page table, and units of a cache head in all, are 32-bit numbers
     if ((int64_t)a->max_pages * ps > 0x7fffff00 || (int64_t)a->max_prefix_pages * ps > 0x7fffff00) return B200_LORA_ERR_DIM;
     const int64_t steps = ((int64_t)a->max_pages * ps + kAttnKeys - 1) / kAttnKeys, psteps = ((int64_t)a->max_prefix_pages * ps + kAttnKeys - 1) / kAttnKeys;
-    if (steps * p.req_tiles * a->n_requests + psteps * p.max_group_tiles > 0x7fffffff) return B200_LORA_ERR_DIM;
+    if (steps * p.req_tiles * a->n_requests + psteps * p.max_group_tiles > 0x7fffffff ||
+        (psteps / (kWideKeys / kAttnKeys) + 1) * p.wide_tiles > 0x7fffffff)
+        return B200_LORA_ERR_DIM;
     if (!aligned16(a->q) || !aligned16(a->out) || !aligned16(cache->k) || !aligned16(cache->v) || !aligned16(workspace) ||
         !rows16(a->q_row, a->q_head) || !rows16(a->out_row, a->out_head) || !rows16(cache->page_stride, cache->token_stride) ||
         cache->head_stride % 8 != 0)
@@ -87,11 +97,14 @@ extern "C" int b200_prefix_attention(const b200_attention* a, const b200_kv_cach
     if (workspace_bytes < attention_bytes(p)) return B200_LORA_ERR_WORKSPACE;
     while ((1 << p.page_shift) < ps) ++p.page_shift;
     p.scale_log2 = a->scale * 1.44269504088896341f;
-    const size_t rows = attn_rows(p);
+    if (p.scale_log2 == 0.f) p.scale_log2 = FLT_MIN;           // equal weights as before, but what is masked stays at -infinity
+    const size_t rows = attn_group_rows(p) + attn_request_rows(p) + attn_wide_rows(p);
     p.part = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part + rows * cache->head_dim);
     p.units = reinterpret_cast<int*>(p.part_ml + rows);
     p.tiles = p.units + a->n_groups + a->n_requests + 1;
+    p.wide_units = p.tiles + a->n_groups + 1;
+    p.wide_tile = p.wide_units + a->n_groups + 1;
     const cudaError_t e = launch_attention(p, dtype, sm_count(), static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? B200_LORA_OK : cuda_fail(e);
 }

@@ -18,6 +18,11 @@ cudaError_t launch_kv_append(const b200_append& a, const b200_kv_cache& c, int d
 constexpr int kAttnKeys = 16;
 constexpr int kAttnRows = 16;
 constexpr int kAttnMaxWorkers = 2048;
+// Groups of more than kAttnRows rows go to the wide kernel: units of kWideKeys keys for tiles of kWideRows rows, one
+// worker per SM.
+constexpr int kWideKeys = 128;
+constexpr int kWideRows = 256;
+constexpr int kWideMaxWorkers = 256;
 
 struct AttnParams {
     b200_attention a;
@@ -28,19 +33,26 @@ struct AttnParams {
     int req_rows;          // rows of a request's partial result
     int max_group_tiles;   // of all groups together
     int workers;
+    int wide_tiles;        // at most, of all groups together; 0: no group can be that large
+    int wide_workers;
     float scale_log2;
     int* units;            // [n_groups + n_requests + 1] units of a cache head before each entity
     int* tiles;            // [n_groups + 1] row tiles before each group
+    int *wide_units, *wide_tile;   // the same of the wide kernel, [n_groups + 1] both
     float* part;           // partial results: rows of head_dim sums, then of (maximum, sum)
     float2* part_ml;
 };
-// rows of partial results: those of the groups' items, then those of the requests'
+// rows of partial results: those of the groups' items, of the requests', of the wide kernel's
 __host__ __device__ inline size_t attn_group_rows(const AttnParams& p) {
     return p.max_group_tiles == 0 ? 0 : ((size_t)p.max_group_tiles * p.c.n_kv_heads + kAttnMaxWorkers) * kAttnRows;
 }
-__host__ __device__ inline size_t attn_rows(const AttnParams& p) {
-    return attn_group_rows(p) + ((size_t)p.a.n_requests * p.req_tiles * p.c.n_kv_heads + kAttnMaxWorkers) * p.req_rows;
+__host__ __device__ inline size_t attn_request_rows(const AttnParams& p) {
+    return ((size_t)p.a.n_requests * p.req_tiles * p.c.n_kv_heads + kAttnMaxWorkers) * p.req_rows;
 }
+__host__ __device__ inline size_t attn_wide_rows(const AttnParams& p) {
+    return p.wide_tiles == 0 ? 0 : ((size_t)p.wide_tiles * p.c.n_kv_heads + kWideMaxWorkers) * kWideRows;
+}
+cudaError_t launch_attention_wide(const AttnParams& p, int dtype, cudaStream_t s);
 cudaError_t launch_attention(const AttnParams& p, int dtype, int n_sm, cudaStream_t s);
 
 // ---- products with 4-bit weights --------------------------------------------------------------

@@ -243,6 +243,17 @@ def test_attention_large_groups(hq, hk, B, plen, d, dtype):
     check_attend(attend_case(B, B, hq, hk, d, 16, dtype, lens, starts=[0, B - 3, B - 1], plens=[plen, 64]))
 
 
+@pytest.mark.parametrize("B,hq,hk,starts,plens", [
+    (93, 40, 40, [0, 18, 40, 57, 93], [1999, 130, 700, 128]),      # more parts of a few blocks, some of one, than SMs
+    (160, 32, 8, [0, 20, 160], [300, 1100]),                       # tiles of one stream's rows, of both and of a rest
+    (64, 64, 64, [0, 20, 40, 64], [1, 129, 257]),                  # one block per item: the second stream has none
+    (70, 16, 2, [0, 35, 70], [4000, 5000])])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_attention_large_groups_of_many_items(B, hq, hk, starts, plens, dtype):
+    check_attend(attend_case(B, B, hq, hk, 128, 16, dtype, np.arange(B) % 7, starts=starts, plens=plens))
+    check_attend(attend_case(B, B, hq, hk, 64, 1, dtype, np.arange(B) % 5, starts=starts, plens=plens))
+
+
 def test_attention_one_long_request_is_split():
     check_attend(attend_case(3, 1, 8, 1, 128, 16, "bf16", [20011]))
     check_attend(attend_case(4, 2, 4, 4, 64, 1, "fp16", [9001, 1]))
@@ -251,6 +262,7 @@ def test_attention_one_long_request_is_split():
 def test_attention_scales_and_large_scores():
     """Scores far from zero, of one sign and of both; a scale of zero and a negative one."""
     for std, scale in ((30.0, None), (1.0, 0.0), (2.0, -0.3)):
+        check_attend(attend_case(6, 40, 8, 2, 64, 16, "fp16", [1] * 40, starts=[0, 39], plens=[700], std=std), scale=scale)
         check_attend(attend_case(5, 5, 8, 2, 64, 16, "bf16", [100, 3, 65, 1, 0], starts=[0, 3], plens=[300], std=std), scale=scale)
 
 
@@ -284,6 +296,9 @@ def test_attention_leaves_bad_pages_lengths_and_groups_out_and_reports_them():
     def case():
         return attend_case(9, 6, 8, 2, 128, 16, "bf16", [100, 30, 65, 1, 0, 64], starts=[0, 2, 5], plens=[90, 127], fill=0.0)
 
+    wide = attend_case(9, 40, 8, 2, 128, 16, "bf16", [3] * 40, starts=[0, 39], plens=[700], fill=0.0)
+    wide["prefix_table"][0, 3], wide["prefix_table"][0, 20] = 10 ** 6, -1
+    check_attend(wide, expect_status=decode.BAD_PAGE)
     for name, where, value in (("block_table", (0, 2), -1), ("block_table", (2, 0), 10 ** 6), ("prefix_table", (1, 3), -2 ** 31 + 1)):
         s = case()
         s[name][where] = value
