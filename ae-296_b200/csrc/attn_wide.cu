@@ -50,6 +50,7 @@ struct WideShared {
     int bad, pad;
 };
 static_assert(sizeof(WideShared) % 16 == 0, "the scan's arrays follow");
+constexpr int kNoPage = -0x7fffffff - 1;         // of a key behind the prefix
 constexpr int kSmemLimit = 232448;                // of a block
 
 __device__ __forceinline__ void tmem_alloc(unsigned smem_dst) {
@@ -65,15 +66,25 @@ __device__ __forceinline__ void tc_commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// D = A B^T, A and B from shared memory
-__device__ __forceinline__ void mma_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, unsigned accumulate) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// Shared-memory operands with 128-byte swizzle: panels of 64 elements, [rows][128 bytes], 16-byte piece c of row r at
+// c ^ (r % 8); 1024 bytes from one eight rows to the next.  Their descriptors as two words, of which only the low one
+// changes: address in units of 16 bytes, and above it for an operand whose rows are the contraction the distance of two panels.
+constexpr unsigned kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+constexpr unsigned kPanel = kStreamRows * 128;                // bytes of a panel of 128 rows
+constexpr unsigned kRowsAreRows = 1u << 16, kRowsAreDepth = (kPanel >> 4) << 16;
+__device__ __forceinline__ unsigned desc_low(unsigned saddr, unsigned kind) { return ((saddr >> 4) & 0x3fffu) | kind; }
+// D (+)= A B^T, A and B from shared memory
+template <bool ACC>
+__device__ __forceinline__ void mma_ss(unsigned d, unsigned a, unsigned b, unsigned idesc) {
+    asm volatile("{ .reg .pred p; .reg .b64 x, y; mov.b64 x, {%1, %3}; mov.b64 y, {%2, %3}; setp.ne.b32 p, %5, 0;"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %4, p; }"
+                 ::"r"(d), "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "n"(ACC) : "memory");
 }
-// D += A B, A from TMEM
-__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, unsigned long long b, unsigned idesc, unsigned accumulate) {
-    asm volatile("{ .reg .pred p; setp.ne.b32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+// D (+)= A B, A from TMEM
+__device__ __forceinline__ void mma_ts(unsigned d, unsigned a, unsigned b, unsigned idesc, unsigned accumulate) {
+    asm volatile("{ .reg .pred p; .reg .b64 y; mov.b64 y, {%2, %3}; setp.ne.b32 p, %5, 0;"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p; }"
+                 ::"r"(d), "r"(a), "r"(b), "r"(kDescHigh), "r"(idesc), "r"(accumulate) : "memory");
 }
 __device__ __forceinline__ void tc_ld32(unsigned taddr, unsigned (&r)[32]) {
     asm volatile(
@@ -103,15 +114,28 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Shared-memory operands with 128-byte swizzle: panels of 64 elements, [rows][128 bytes], 16-byte piece c of row r at
-// c ^ (r % 8).  Rows are rows of the operand (K-major) or the contraction (MN-major: `panel` bytes from one 64 to the next).
-__device__ __forceinline__ unsigned long long desc_k(unsigned saddr) {
-    return (unsigned long long)((saddr >> 4) & 0x3fffu) | (1ull << 16) | ((unsigned long long)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// two fp32 numbers at a time
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
-__device__ __forceinline__ unsigned long long desc_mn(unsigned saddr, unsigned panel) {
-    return (unsigned long long)((saddr >> 4) & 0x3fffu) | ((unsigned long long)(panel >> 4) << 16) | ((unsigned long long)(1024 >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
+__device__ __forceinline__ float2 unpair(unsigned long long v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
 }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // kind::f16, fp32 sums, M = 128; b_mn: the second operand's rows are the contraction
 __device__ __forceinline__ unsigned idesc_of(bool bf16, int n, bool b_mn) {
     const unsigned fmt = bf16 ? 1u : 0u;
@@ -119,7 +143,7 @@ __device__ __forceinline__ unsigned idesc_of(bool bf16, int n, bool b_mn) {
 }
 // byte address of 16-byte piece `piece` of row `row` in an operand of 128 rows
 __device__ __forceinline__ unsigned swizzled(unsigned base, int row, int piece) {
-    return base + (piece >> 3) * (128 * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
+    return base + (piece >> 3) * kPanel + row * 128 + (((piece & 7) ^ (row & 7)) << 4);
 }
 
 // An item's part of a worker: blocks [b0, b0 + n) of tile `tile` of cache head `h` of group `g`.
@@ -204,8 +228,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
 
     if (warp >= 9) {
         // ================= copies =================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int cw = warp - 9;
         constexpr int kPieces = D / 8, kRowsAt = 32 / kPieces;
+        constexpr int kGroups = kWideKeys / kRowsAt, kMine = (kGroups + kCopyWarps - 1) / kCopyWarps;   // a copy's rows; this warp's copies
+        static_assert(kMine * kRowsAt <= 64, "two rows' places a lane");
         const int piece = lane % kPieces, sub = lane / kPieces;
         const int in_page = (1 << p.page_shift) - 1;
         unsigned n = 0, n_keys = 0;              // blocks, and blocks of keys, so far
@@ -216,19 +243,32 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             mbar_arrive(bar(sh.full[pending]));
             pending = -1;
         };
+        // The places of the rows that this warp copies, one or two a lane: row i is row i % kRowsAt of its copy i / kRowsAt.
+        // The page table is read a block ahead, or each copy would wait for it.
+        auto row_of = [&](int i) { return (cw + kCopyWarps * (i / kRowsAt)) * kRowsAt + i % kRowsAt; };
+        int page[2];
         for (long long u = u_first; u < u_end;) {
             const Part t = part_at(u);
             const int* table = p.a.prefix_table + (long long)t.g * p.a.prefix_table_row;
-            for (int i = 0; i < 2 * t.n; ++i, ++n) {
-                bool is_v;
-                int b;
-                if (t.dual) { is_v = i & 1; b = i >> 1; }
-                else {
-                    const int lead = min(2, t.n), j = i - lead, pairs = max(t.n - 2, 0);
-                    if (j < 0) { is_v = false; b = i; }
-                    else if (j < 2 * pairs) { is_v = !(j & 1); b = is_v ? j >> 1 : (j >> 1) + 2; }
-                    else { is_v = true; b = j - pairs; }
+            auto block_at = [&](int i, bool& is_v) {
+                if (t.dual) { is_v = i & 1; return i >> 1; }
+                const int lead = min(2, t.n), j = i - lead, pairs = max(t.n - 2, 0);
+                if (j < 0) { is_v = false; return i; }
+                if (j < 2 * pairs) { is_v = !(j & 1); return is_v ? j >> 1 : (j >> 1) + 2; }
+                is_v = true;
+                return j - pairs;
+            };
+            auto read_table = [&](int b) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int row = row_of(lane + 32 * k), key = (t.b0 + b) * kWideKeys + row;
+                    page[k] = row < kWideKeys && key < t.keys ? __ldg(table + (key >> p.page_shift)) : kNoPage;
                 }
+            };
+            bool is_v, next_v;
+            int b = block_at(0, is_v);
+            read_table(b);
+            for (int i = 0; i < 2 * t.n; ++i, ++n) {
                 const int slot = n % RING;
                 const unsigned phase = ((n / RING) & 1) ^ 1;
                 if (!mbar_try_wait(bar(sh.empty[slot]), phase)) {       // what has arrived meanwhile must not wait for this
@@ -237,96 +277,113 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                     mbar_wait(bar(sh.empty[slot]), phase, err, 1);
                 }
                 __syncwarp();
-                const unsigned dst = ring + slot * W::kBlock;
-                const int key0 = (t.b0 + b) * kWideKeys;
-                const T* base = static_cast<const T*>(is_v ? p.c.v : p.c.k) + (long long)t.h * p.c.head_stride + piece * 8;
-                uint4 missing = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll 4
-                for (int g = cw; g < kWideKeys / kRowsAt; g += kCopyWarps) {
-                    const int row = g * kRowsAt + sub, key = key0 + row;
-                    const bool wanted = key < t.keys;
-                    const int page = wanted ? __ldg(table + (key >> p.page_shift)) : 0;
-                    const bool fine = wanted && (unsigned)page < (unsigned)p.c.n_pages;
-                    const long long at = fine ? (long long)page * p.c.page_stride + (long long)(key & in_page) * p.c.token_stride : 0;
-                    cp_async16(swizzled(dst, row, piece), base + at, fine);
-                    const unsigned lost = __ballot_sync(0xffffffffu, wanted && !fine && piece == 0);
-                    if (lost) {
-                        if (lane == 0 && p.a.status) atomicOr(p.a.status, B200_DECODE_BAD_PAGE);
-                        unsigned rows = 0;
+                long long at[2];                 // < 0: zeros
+                bool lost[2];
 #pragma unroll
-                        for (int k = 0; k < kRowsAt; ++k) rows |= ((lost >> (k * kPieces)) & 1u) << ((g * kRowsAt + k) & 31);
-                        const int word = (g * kRowsAt) >> 5;
-                        missing.x |= word == 0 ? rows : 0u; missing.y |= word == 1 ? rows : 0u;
-                        missing.z |= word == 2 ? rows : 0u; missing.w |= word == 3 ? rows : 0u;
-                    }
+                for (int k = 0; k < 2; ++k) {
+                    const int key = (t.b0 + b) * kWideKeys + row_of(lane + 32 * k);
+                    const bool fine = (unsigned)page[k] < (unsigned)p.c.n_pages;
+                    lost[k] = !fine && page[k] != kNoPage;
+                    at[k] = fine ? (long long)page[k] * p.c.page_stride + (long long)(key & in_page) * p.c.token_stride : -1;
                 }
-                cp_commit();
                 if (!is_v) {
+                    uint4 missing = make_uint4(0u, 0u, 0u, 0u);
+                    if (__any_sync(0xffffffffu, lost[0] || lost[1])) {
+                        if (lane == 0 && p.a.status) atomicOr(p.a.status, B200_DECODE_BAD_PAGE);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int row = row_of(lane + 32 * k);
+                            const unsigned bit = lost[k] ? 1u << (row & 31) : 0u;
+                            missing.x |= row >> 5 == 0 ? bit : 0u; missing.y |= row >> 5 == 1 ? bit : 0u;
+                            missing.z |= row >> 5 == 2 ? bit : 0u; missing.w |= row >> 5 == 3 ? bit : 0u;
+                        }
+                        missing.x = __reduce_or_sync(0xffffffffu, missing.x); missing.y = __reduce_or_sync(0xffffffffu, missing.y);
+                        missing.z = __reduce_or_sync(0xffffffffu, missing.z); missing.w = __reduce_or_sync(0xffffffffu, missing.w);
+                    }
                     if (lane == 0) sh.missing[n_keys % kMissing][cw] = missing;
                     ++n_keys;
                 }
+                int next = 0;
+                if (i + 1 < 2 * t.n) {
+                    next = block_at(i + 1, next_v);
+                    read_table(next);
+                }
+                const unsigned dst = ring + slot * W::kBlock;
+                const T* base = static_cast<const T*>(is_v ? p.c.v : p.c.k) + (long long)t.h * p.c.head_stride + piece * 8;
+#pragma unroll
+                for (int j = 0; j < kMine; ++j) {
+                    const int g = cw + kCopyWarps * j, row = g * kRowsAt + sub;
+                    const long long from = __shfl_sync(0xffffffffu, at[j * kRowsAt >= 32], (j * kRowsAt + sub) & 31);
+                    if (g < kGroups) cp_async16(swizzled(dst, row, piece), base + max(from, 0ll), from >= 0);
+                }
+                cp_commit();
                 if (pending >= 0) { cp_wait<1>(); arrived(); }
                 pending = slot;
+                b = next;
+                is_v = next_v;
             }
             u += t.n;
         }
         cp_wait<0>();
         arrived();
     } else if (warp == 8) {
-        // ================= multiplications =================
-        const bool bf16 = Cvt<T>::is_bf16;
-        const unsigned id_s = idesc_of(bf16, kWideKeys, false), id_o = idesc_of(bf16, D, true);
-        unsigned n = 0, parts[2] = {0u, 0u}, rounds[2] = {0u, 0u};       // blocks, each stream's parts and rounds so far
-        for (long long u = u_first; u < u_end;) {
-            const Part t = part_at(u);
-            auto block_of = [&](int s, int r) { return t.dual ? r : 2 * r + s; };
-            auto wait_full = [&](int at) { const unsigned k = n + at; mbar_wait(bar(sh.full[k % RING]), (k / RING) & 1, err, 2); tc_fence_after(); };
-            auto scores = [&](int s, int b) {
-                const int at = k_at(t, b);
-                wait_full(at);
-                if (lane == 0) {
-                    const unsigned slot = (n + at) % RING, ka = ring + slot * W::kBlock, qa = smem_u32(smem) + s * W::kQ;
+        // ================= multiplications: one thread =================
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (lane == 0) {
+            const unsigned id_s = idesc_of(Cvt<T>::is_bf16, kWideKeys, false), id_o = idesc_of(Cvt<T>::is_bf16, D, true);
+            const unsigned q_low = desc_low(smem_u32(smem), kRowsAreRows);
+            unsigned n = 0, q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};      // n: blocks before this part
+            for (long long u = u_first; u < u_end;) {
+                const Part t = part_at(u);
+                const int take = t.dual ? 1 : 2;                 // from one block of a stream to its next
+                auto wait_full = [&](unsigned k) { mbar_wait(bar(sh.full[k % RING]), (k / RING) & 1, err, 2); };
+                auto scores = [&](int s, int b) {
+                    const unsigned k = n + k_at(t, b), slot = k % RING;
+                    wait_full(k);
+                    tc_fence_after();
+                    const unsigned qa = q_low + s * (W::kQ >> 4), ka = desc_low(ring + slot * W::kBlock, kRowsAreRows);
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const unsigned off = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                        mma_ss(tmem + s * 128, desc_k(qa + off), desc_k(ka + off), id_s, k != 0);
+                    for (int i = 0; i < D / 16; ++i) {
+                        const unsigned off = ((i >> 2) * kPanel + (i & 3) * 32) >> 4;
+                        if (i == 0) mma_ss<false>(tmem + s * 128, qa, ka, id_s);
+                        else mma_ss<true>(tmem + s * 128, qa + off, ka + off, id_s);
                     }
                     tc_commit(bar(sh.s_full[s]));
                     if (!t.dual || s == 1) tc_commit(bar(sh.empty[slot]));
-                }
-                __syncwarp();
-            };
-            for (int s = 0; s < 2; ++s)
-                if (block_of(s, 0) < t.n) {                      // a stream without a block has no queries either
-                    mbar_wait(bar(sh.q_ready[s]), parts[s] & 1, err, 3);
-                    ++parts[s];
-                    tc_fence_after();
-                    scores(s, block_of(s, 0));
-                }
-            for (int r = 0; block_of(0, r) < t.n; ++r)
+                };
                 for (int s = 0; s < 2; ++s) {
-                    const int b = block_of(s, r);
-                    if (b >= t.n) continue;
-                    mbar_wait(bar(sh.p_ready[s]), rounds[s] & 1, err, 4);
-                    ++rounds[s];
-                    const int at = v_at(t, b);
-                    wait_full(at);
-                    if (lane == 0) {
-                        const unsigned slot = (n + at) % RING, va = ring + slot * W::kBlock;
-#pragma unroll
-                        for (int k = 0; k < kWideKeys / 16; ++k)
-                            mma_ts(tmem + 256 + s * 128, tmem + s * 128 + k * 8, desc_mn(va + k * 2048, 128 * 128), id_o, (r | k) != 0);
-                        if (!t.dual || s == 1) tc_commit(bar(sh.empty[slot]));
-                        if (block_of(s, r + 1) >= t.n) tc_commit(bar(sh.o_full[s]));
-                    }
-                    __syncwarp();
-                    if (block_of(s, r + 1) < t.n) scores(s, block_of(s, r + 1));
+                    const int b = t.dual ? 0 : s;
+                    if (b >= t.n) continue;                      // a stream without a block has no queries either
+                    mbar_wait(bar(sh.q_ready[s]), q_phase[s], err, 3);
+                    q_phase[s] ^= 1;
+                    scores(s, b);
                 }
-            n += 2 * t.n;
-            u += t.n;
+                for (int r = 0; r < t.n; r += take)
+                    for (int s = 0; s < 2; ++s) {
+                        const int b = t.dual ? r : r + s;
+                        if (b >= t.n) continue;
+                        const unsigned k = n + v_at(t, b), slot = k % RING;
+                        wait_full(k);
+                        mbar_wait(bar(sh.p_ready[s]), p_phase[s], err, 4);
+                        p_phase[s] ^= 1;
+                        tc_fence_after();
+                        const unsigned va = desc_low(ring + slot * W::kBlock, kRowsAreDepth);
+#pragma unroll
+                        for (int i = 0; i < kWideKeys / 16; ++i)
+                            mma_ts(tmem + 256 + s * 128, tmem + s * 128 + i * 8, va + i * (2048 >> 4), id_o, i > 0 || r > 0);
+                        if (b + take >= t.n) tc_commit(bar(sh.o_full[s]));
+                        if (!t.dual || s == 1) tc_commit(bar(sh.empty[slot]));
+                        if (b + take < t.n) scores(s, b + take);
+                    }
+                n += 2 * t.n;
+                u += t.n;
+            }
         }
+        __syncwarp();
     } else {
         // ================= the streams =================
+        // 256 * 208 + 128 * 80 registers: no more than the 384 * 168 of the launch
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int s = warp >> 2, row = tid & 127;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const unsigned s_tm = tmem + lanes + s * 128, o_tm = tmem + lanes + 256 + s * 128;
@@ -378,7 +435,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                     }
                     float x[4] = {z(0), z(1), z(2), z(3)};
 #pragma unroll
-                    for (int j = 4; j < 128; ++j) x[j & 3] = fmaxf(x[j & 3], z(j));
+                    for (int j = 4; j < 124; j += 8)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) x[i] = fmaxf(fmaxf(x[i], z(j + i)), z(j + 4 + i));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = fmaxf(x[i], z(124 + i));
                     const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * scale;
                     if (b == b_first) m = top;
                     else {
@@ -400,20 +461,23 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : m - kLift;      // nothing yet: every weight is 0
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const unsigned long long scale2 = pair(scale, scale), ref2 = pair(-ref, -ref);
+                    unsigned long long sum[2] = {0ull, 0ull};
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         unsigned w[32];
 #pragma unroll
                         for (int j = 0; j < 32; ++j) {
-                            const float a = ex2(fmaf(z(c * 64 + 2 * j), scale, -ref)), d = ex2(fmaf(z(c * 64 + 2 * j + 1), scale, -ref));
-                            sum[(2 * j) & 3] += a;
-                            sum[(2 * j + 1) & 3] += d;
-                            w[j] = Cvt<T>::pack2(a, d);
+                            float2 e = unpair(fma2(pair(z(c * 64 + 2 * j), z(c * 64 + 2 * j + 1)), scale2, ref2));
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                            sum[j & 1] = add2(sum[j & 1], pair(e.x, e.y));
+                            w[j] = Cvt<T>::pack2(e.x, e.y);
                         }
                         tc_st32(s_tm + c * 32, w);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    const float2 sums = unpair(add2(sum[0], sum[1]));
+                    l += sums.x + sums.y;
                     tc_wait_st();
                 }
                 tc_fence_before();
