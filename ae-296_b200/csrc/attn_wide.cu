@@ -66,6 +66,11 @@ __device__ __forceinline__ void tc_commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// one of the barrier's arrivals, once this thread's copies so far have landed
+__device__ __forceinline__ void arrive_when_copied(unsigned b) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(b) : "memory");
+}
+__device__ __forceinline__ void cp_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Shared-memory operands with 128-byte swizzle: panels of 64 elements, [rows][128 bytes], 16-byte piece c of row r at
 // c ^ (r % 8); 1024 bytes from one eight rows to the next.  Their descriptors as two words, of which only the low one
 // changes: address in units of 16 bytes, and above it for an operand whose rows are the contraction the distance of two panels.
@@ -105,6 +110,12 @@ __device__ __forceinline__ void tc_st32(unsigned taddr, const unsigned (&r)[32])
           "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
           "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tc_st16(unsigned taddr, const unsigned (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+                   "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -222,13 +233,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&sh.tmem);
     const unsigned ring = smem_u32(smem) + 2 * W::kQ;
     // The ring's order within a part: where the streams share blocks, K0 V0 K1 V1 ...; where they take them in turns,
-    // K0 K1 V0 K2 V1 K3 ...: what the multiplications wait for next always comes next.
-    auto k_at = [](const Part& t, int b) { return t.dual ? 2 * b : b < 2 ? b : 2 * b - 1; };
-    auto v_at = [](const Part& t, int b) { return t.dual ? 2 * b + 1 : min(2, t.n) + b + min(b, max(t.n - 2, 0)); };
-
+    // K0 K1 V0 K2 V1 K3 ...: what the multiplications need next always comes next.
     if (warp >= 9) {
         // ================= copies =================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         const int cw = warp - 9;
         constexpr int kPieces = D / 8, kRowsAt = 32 / kPieces;
         constexpr int kGroups = kWideKeys / kRowsAt, kMine = (kGroups + kCopyWarps - 1) / kCopyWarps;   // a copy's rows; this warp's copies
@@ -236,13 +243,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
         const int piece = lane % kPieces, sub = lane / kPieces;
         const int in_page = (1 << p.page_shift) - 1;
         unsigned n = 0, n_keys = 0;              // blocks, and blocks of keys, so far
-        int pending = -1;                        // slot whose copies are in flight
-        auto arrived = [&]() {
-            if (pending < 0) return;
-            fence_async_proxy();                 // the copies wrote through the generic proxy
-            mbar_arrive(bar(sh.full[pending]));
-            pending = -1;
-        };
         // The places of the rows that this warp copies, one or two a lane: row i is row i % kRowsAt of its copy i / kRowsAt.
         // The page table is read a block ahead, or each copy would wait for it.
         auto row_of = [&](int i) { return (cw + kCopyWarps * (i / kRowsAt)) * kRowsAt + i % kRowsAt; };
@@ -270,12 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             read_table(b);
             for (int i = 0; i < 2 * t.n; ++i, ++n) {
                 const int slot = n % RING;
-                const unsigned phase = ((n / RING) & 1) ^ 1;
-                if (!mbar_try_wait(bar(sh.empty[slot]), phase)) {       // what has arrived meanwhile must not wait for this
-                    cp_wait<0>();
-                    arrived();
-                    mbar_wait(bar(sh.empty[slot]), phase, err, 1);
-                }
+                mbar_wait(bar(sh.empty[slot]), ((n / RING) & 1) ^ 1, err, 1);
                 __syncwarp();
                 long long at[2];                 // < 0: zeros
                 bool lost[2];
@@ -316,74 +311,80 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                     const long long from = __shfl_sync(0xffffffffu, at[j * kRowsAt >= 32], (j * kRowsAt + sub) & 31);
                     if (g < kGroups) cp_async16(swizzled(dst, row, piece), base + max(from, 0ll), from >= 0);
                 }
-                cp_commit();
-                if (pending >= 0) { cp_wait<1>(); arrived(); }
-                pending = slot;
+                arrive_when_copied(bar(sh.full[slot]));
                 b = next;
                 is_v = next_v;
             }
             u += t.n;
         }
-        cp_wait<0>();
-        arrived();
+        cp_wait_all();
     } else if (warp == 8) {
         // ================= multiplications: one thread =================
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
         if (lane == 0) {
             const unsigned id_s = idesc_of(Cvt<T>::is_bf16, kWideKeys, false), id_o = idesc_of(Cvt<T>::is_bf16, D, true);
-            const unsigned q_low = desc_low(smem_u32(smem), kRowsAreRows);
-            unsigned n = 0, q_phase[2] = {0u, 0u}, p_phase[2] = {0u, 0u};      // n: blocks before this part
+            const unsigned q_low = desc_low(smem_u32(smem), kRowsAreRows), full0 = bar(sh.full[0]), empty0 = bar(sh.empty[0]);
+            const unsigned q0 = bar(sh.q_ready[0]), s0 = bar(sh.s_full[0]), p0 = bar(sh.p_ready[0]), o0 = bar(sh.o_full[0]);
+            unsigned slot = 0, phase = 0;                        // of the block that is needed next: the ring's order is theirs
+            unsigned q_phase = 0, p_phase = 0;                   // bit s: of stream s
+            auto next_block = [&]() {                            // waits for it and returns its slot
+                const unsigned at = slot;
+                mbar_wait(full0 + at * 8, phase, err, 2);
+                fence_async_proxy();                             // the copies wrote through the generic proxy
+                if (++slot == RING) { slot = 0; phase ^= 1; }
+                return at;
+            };
+            auto scores = [&](int s, unsigned k, bool last_use) {
+                tc_fence_after();
+                const unsigned qa = q_low + s * (W::kQ >> 4), ka = desc_low(ring + k * W::kBlock, kRowsAreRows), d = tmem + s * 128;
+                mma_ss<false>(d, qa, ka, id_s);
+#pragma unroll
+                for (int i = 1; i < D / 16; ++i) {
+                    const unsigned off = ((i >> 2) * kPanel + (i & 3) * 32) >> 4;
+                    mma_ss<true>(d, qa + off, ka + off, id_s);
+                }
+                tc_commit(s0 + s * 8);
+                if (last_use) tc_commit(empty0 + k * 8);
+            };
+            auto queries = [&](int s) { mbar_wait(q0 + s * 8, q_phase >> s & 1, err, 3); q_phase ^= 1u << s; };
+            auto weigh = [&](int s, unsigned v, bool first, bool last, bool last_use) {
+                mbar_wait(p0 + s * 8, p_phase >> s & 1, err, 4);
+                p_phase ^= 1u << s;
+                tc_fence_after();
+                const unsigned va = desc_low(ring + v * W::kBlock, kRowsAreDepth), d = tmem + 256 + s * 128, w = tmem + s * 128;
+                mma_ts(d, w, va, id_o, !first);
+#pragma unroll
+                for (int i = 1; i < kWideKeys / 16; ++i) mma_ts(d, w + i * 8, va + i * (2048 >> 4), id_o, 1);
+                if (last) tc_commit(o0 + s * 8);
+                if (last_use) tc_commit(empty0 + v * 8);
+            };
             for (long long u = u_first; u < u_end;) {
                 const Part t = part_at(u);
-                const int take = t.dual ? 1 : 2;                 // from one block of a stream to its next
-                auto wait_full = [&](unsigned k) { mbar_wait(bar(sh.full[k % RING]), (k / RING) & 1, err, 2); };
-                auto scores = [&](int s, int b) {
-                    const unsigned k = n + k_at(t, b), slot = k % RING;
-                    wait_full(k);
-                    tc_fence_after();
-                    const unsigned qa = q_low + s * (W::kQ >> 4), ka = desc_low(ring + slot * W::kBlock, kRowsAreRows);
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i) {
-                        const unsigned off = ((i >> 2) * kPanel + (i & 3) * 32) >> 4;
-                        if (i == 0) mma_ss<false>(tmem + s * 128, qa, ka, id_s);
-                        else mma_ss<true>(tmem + s * 128, qa + off, ka + off, id_s);
+                const int n = t.n;
+                if (t.dual) {
+                    unsigned k = next_block();
+                    for (int s = 0; s < 2; ++s) { queries(s); scores(s, k, s == 1); }
+                    for (int b = 0; b < n; ++b) {
+                        const unsigned v = next_block();
+                        const bool more = b + 1 < n;
+                        weigh(0, v, b == 0, !more, false);
+                        if (more) { k = next_block(); scores(0, k, false); }
+                        weigh(1, v, b == 0, !more, true);
+                        if (more) scores(1, k, true);
                     }
-                    tc_commit(bar(sh.s_full[s]));
-                    if (!t.dual || s == 1) tc_commit(bar(sh.empty[slot]));
-                };
-                for (int s = 0; s < 2; ++s) {
-                    const int b = t.dual ? 0 : s;
-                    if (b >= t.n) continue;                      // a stream without a block has no queries either
-                    mbar_wait(bar(sh.q_ready[s]), q_phase[s], err, 3);
-                    q_phase[s] ^= 1;
-                    scores(s, b);
+                } else {
+                    for (int s = 0; s < 2 && s < n; ++s) { queries(s); scores(s, next_block(), true); }
+                    for (int b = 0; b < n; ++b) {
+                        const bool more = b + 2 < n;
+                        weigh(b & 1, next_block(), b < 2, !more, true);
+                        if (more) scores(b & 1, next_block(), true);
+                    }
                 }
-                for (int r = 0; r < t.n; r += take)
-                    for (int s = 0; s < 2; ++s) {
-                        const int b = t.dual ? r : r + s;
-                        if (b >= t.n) continue;
-                        const unsigned k = n + v_at(t, b), slot = k % RING;
-                        wait_full(k);
-                        mbar_wait(bar(sh.p_ready[s]), p_phase[s], err, 4);
-                        p_phase[s] ^= 1;
-                        tc_fence_after();
-                        const unsigned va = desc_low(ring + slot * W::kBlock, kRowsAreDepth);
-#pragma unroll
-                        for (int i = 0; i < kWideKeys / 16; ++i)
-                            mma_ts(tmem + 256 + s * 128, tmem + s * 128 + i * 8, va + i * (2048 >> 4), id_o, i > 0 || r > 0);
-                        if (b + take >= t.n) tc_commit(bar(sh.o_full[s]));
-                        if (!t.dual || s == 1) tc_commit(bar(sh.empty[slot]));
-                        if (b + take < t.n) scores(s, b + take);
-                    }
-                n += 2 * t.n;
-                u += t.n;
+                u += n;
             }
         }
         __syncwarp();
     } else {
         // ================= the streams =================
-        // 256 * 208 + 128 * 80 registers: no more than the 384 * 168 of the launch
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
         const int s = warp >> 2, row = tid & 127;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const unsigned s_tm = tmem + lanes + s * 128, o_tm = tmem + lanes + 256 + s * 128;
@@ -416,30 +417,33 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             float m = -INFINITY, l = 0.f;                        // sums are relative to 2^(m - kLift)
             for (int b = b_first; b < t.n; b += step, ++rounds) {
                 mbar_wait(bar(sh.s_full[s]), rounds & 1, err, 5);
+                __syncwarp();                                    // lanes may leave a wait one by one: what follows is for whole warps
                 tc_fence_after();
                 if (warp_live) {
-                    unsigned zr[4][32];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tc_ld32(s_tm + c * 32, zr[c]);
-                    auto z = [&](int j) { return __uint_as_float(zr[j >> 5][j & 31]); };
-                    tc_wait_ld();
                     // keys behind the prefix, or in pages that do not exist
                     const uint4* lost = sh.missing[(n_keys + b) % kMissing];
                     const uint4 w0 = lost[0], w1 = lost[1], w2 = lost[2];
                     const int valid = t.keys - (t.b0 + b) * kWideKeys;
-                    if (valid < kWideKeys || ((w0.x | w1.x | w2.x) | (w0.y | w1.y | w2.y) | (w0.z | w1.z | w2.z) | (w0.w | w1.w | w2.w))) {
-                        const unsigned gone[4] = {w0.x | w1.x | w2.x, w0.y | w1.y | w2.y, w0.z | w1.z | w2.z, w0.w | w1.w | w2.w};
+                    const unsigned gone[4] = {w0.x | w1.x | w2.x, w0.y | w1.y | w2.y, w0.z | w1.z | w2.z, w0.w | w1.w | w2.w};
+                    const bool masked = valid < kWideKeys || (gone[0] | gone[1] | gone[2] | gone[3]);
+                    auto mask = [&](unsigned (&z)[32], int c) {
 #pragma unroll
-                        for (int j = 0; j < 128; ++j)
-                            if (j >= valid || (gone[j >> 5] >> (j & 31) & 1u)) zr[j >> 5][j & 31] = 0xff800000u;      // -infinity
+                        for (int j = 0; j < 32; ++j)
+                            if (c * 32 + j >= valid || (gone[c] >> j & 1u)) z[j] = 0xff800000u;      // -infinity
+                    };
+                    // The scores are read twice, 32 at a time, for their maximum and for the weights: a row of them would
+                    // leave no registers.
+                    float x[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int c = 0; c < 4; c += 2) {
+                        unsigned za[32], zb[32];
+                        tc_ld32(s_tm + c * 32, za);
+                        tc_ld32(s_tm + c * 32 + 32, zb);
+                        tc_wait_ld();
+                        if (masked) { mask(za, c); mask(zb, c + 1); }
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) x[j & 3] = fmaxf(fmaxf(x[j & 3], __uint_as_float(za[j])), __uint_as_float(zb[j]));
                     }
-                    float x[4] = {z(0), z(1), z(2), z(3)};
-#pragma unroll
-                    for (int j = 4; j < 124; j += 8)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[i] = fmaxf(fmaxf(x[i], z(j + i)), z(j + 4 + i));
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = fmaxf(x[i], z(124 + i));
                     const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * scale;
                     if (b == b_first) m = top;
                     else {
@@ -463,18 +467,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                     const float ref = m == -INFINITY ? 0.f : m - kLift;      // nothing yet: every weight is 0
                     const unsigned long long scale2 = pair(scale, scale), ref2 = pair(-ref, -ref);
                     unsigned long long sum[2] = {0ull, 0ull};
+                    unsigned z[2][32];
+                    tc_ld32(s_tm, z[0]);
+                    tc_wait_ld();
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        unsigned w[32];
+                    for (int c = 0; c < 4; ++c) {
+                        // the weights' words lie where the scores of the first half lay: read what is still needed first
+                        if (c < 3) tc_ld32(s_tm + (c + 1) * 32, z[(c + 1) & 1]);
+                        if (masked) mask(z[c & 1], c);
+                        unsigned w[16];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            float2 e = unpair(fma2(pair(z(c * 64 + 2 * j), z(c * 64 + 2 * j + 1)), scale2, ref2));
+                        for (int j = 0; j < 16; ++j) {
+                            float2 e = unpair(fma2(pair(__uint_as_float(z[c & 1][2 * j]), __uint_as_float(z[c & 1][2 * j + 1])), scale2, ref2));
                             e.x = ex2(e.x);
                             e.y = ex2(e.y);
                             sum[j & 1] = add2(sum[j & 1], pair(e.x, e.y));
                             w[j] = Cvt<T>::pack2(e.x, e.y);
                         }
-                        tc_st32(s_tm + c * 32, w);
+                        if (c < 3) tc_wait_ld();
+                        tc_st16(s_tm + c * 16, w);
                     }
                     const float2 sums = unpair(add2(sum[0], sum[1]));
                     l += sums.x + sums.y;
@@ -488,6 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             if (b_first < t.n) {
                 mbar_wait(bar(sh.o_full[s]), outs & 1, err, 6);
                 ++outs;
+                __syncwarp();
                 tc_fence_after();
                 if (warp_live) {
                     float* dst = p.part + out_row * D;
