@@ -114,9 +114,11 @@ extern "C" int b200_int4_linear(const b200_int4* a, int32_t dtype, int32_t y_dty
     if (!io_type(dtype) || (y_dtype != dtype && y_dtype != B200_LORA_F32)) return B200_LORA_ERR_DTYPE;
     if (a->n_tokens < 0 || a->n_in < 1 || a->n_out < 1 || (a->group != 32 && a->group != 64 && a->group != 128) || a->n_in % a->group != 0)
         return B200_LORA_ERR_DIM;
-    if (!aligned16(a->x) || !aligned16(a->codes) || a->x_row % 8 != 0) return B200_LORA_ERR_ALIGN;
+    if (!aligned16(a->x) || !aligned16(a->codes) || (a->n_tokens > 1 && a->x_row % 8 != 0)) return B200_LORA_ERR_ALIGN;
     if (a->n_tokens == 0) return B200_LORA_OK;
-    if ((int64_t)a->n_tokens > 65535 * 32) return B200_LORA_ERR_DIM;
-    const cudaError_t e = launch_int4(*a, dtype, y_dtype == B200_LORA_F32, sm_count(), static_cast<cudaStream_t>(stream));
+    b200_int4 q = *a;
+    if (a->n_tokens == 1) q.x_row = (a->n_in + 7) / 8 * 8;       // whatever it was said to be
+    if (q.x_row < a->n_in || a->n_tokens > 65535 * 64) return B200_LORA_ERR_DIM;
+    const cudaError_t e = launch_int4(q, dtype, y_dtype == B200_LORA_F32, sm_count(), static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? B200_LORA_OK : cuda_fail(e);
 }

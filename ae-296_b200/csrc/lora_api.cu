@@ -52,6 +52,28 @@ EncodeTiledFn encode_tiled() {
     return fn;
 }
 
+}  // namespace
+
+// Map over 16-bit numbers with boxes of 128-byte swizzled rows: extents and box from the contiguous dimension on, strides in
+// elements from the second on
+bool b200lora::encode_map(CUtensorMap* out, const void* base, std::initializer_list<uint64_t> extents, std::initializer_list<uint64_t> strides,
+                          std::initializer_list<uint32_t> box) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return false;
+    cuuint64_t dims[3], pitch[3];
+    cuuint32_t sides[3], ones[3] = {1, 1, 1};
+    int n = 0;
+    for (uint64_t e : extents) dims[n++] = e;
+    n = 0;
+    for (uint64_t e : strides) pitch[n++] = e * 2;
+    n = 0;
+    for (uint32_t e : box) sides[n++] = e;
+    return fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT16, (cuuint32_t)n, const_cast<void*>(base), dims, pitch, sides, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+namespace {
+
 // 2-D map over a row-major 16-bit matrix [rows, inner] with row pitch `pitch` elements;
 // cached per (base, shape, box)
 bool tensor_map_2d(CUtensorMap* out, const void* base, uint64_t inner, uint64_t rows, uint32_t box_inner,

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
 #include <utility>
 
 #include "b200_lora.h"
@@ -305,6 +306,8 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
 // ---- shared by the entry points (lora_api.cu) ------------------------------------------------
 int cuda_fail(cudaError_t e);             // keeps the error's text for b200_lora_last_cuda_error; returns B200_LORA_ERR_CUDA
 int sm_count();                           // of the current device
+bool encode_map(CUtensorMap* out, const void* base, std::initializer_list<uint64_t> extents, std::initializer_list<uint64_t> strides,
+                std::initializer_list<uint32_t> box);
 
 // ---- launchers implemented by the kernel files ---------------------------------------------
 struct PlanAdapters {          // what the plan bakes into its unit records

@@ -95,7 +95,7 @@ int b200_prefix_attention(const b200_attention* a, const b200_kv_cache* cache, i
  * codes [n_out, n_in / 2] bytes: column 2 i in the low four bits of byte i, column 2 i + 1 in the high ones.
  * scales [n_out, n_in / group] of x's type; zeros (NULL: 8 everywhere) [n_out, n_in / group] bytes, of which the low
  * four bits count; both contiguous.  group is 32, 64 or 128 and divides n_in.  x [n_tokens, n_in] and y
- * [n_tokens, n_out] with row strides; y and add are of x's type or both fp32; add (NULL: none) may be y.  Any number of
+ * [n_tokens, n_out] with row strides (x's rows do not overlap); y and add are of x's type or both fp32; add (NULL: none) may be y.  Any number of
  * tokens; made for the few of a decode step. */
 typedef struct b200_int4 {
     void* y;
