@@ -432,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
 template <typename T, int D, int RING>
 cudaError_t launch_ring(const AttnParams& p, size_t scan, cudaStream_t s) {
     const size_t smem = Wide<D, RING>::kBytes + sizeof(WideShared) + scan + 1024;
-    const cudaError_t e = cudaFuncSetAttribute(attn_wide_kernel<T, D, RING>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = allow_smem<attn_wide_kernel<T, D, RING>>((int)smem);
     if (e != cudaSuccess) return e;
     return launch_pdl(attn_wide_kernel<T, D, RING>, p.wide_workers, kThreads, smem, s, p);
 }

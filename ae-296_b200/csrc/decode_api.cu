@@ -59,7 +59,7 @@ extern "C" int b200_kv_append(const b200_append* a, const b200_kv_cache* cache, 
     if (a->dq) vec = vec && aligned16(a->dq) && rows16(a->dq_row, a->dq_head);
     if (a->dk) vec = vec && aligned16(a->dk) && rows16(a->dk_row, a->dk_head);
     if (a->dv) vec = vec && aligned16(a->dv) && rows16(a->dv_row, a->dv_head);
-    const cudaError_t e = launch_kv_append(*a, *cache, dtype, vec, static_cast<cudaStream_t>(stream));
+    const cudaError_t e = launch_kv_append(*a, *cache, dtype, vec, sm_count(), static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? B200_LORA_OK : cuda_fail(e);
 }
 

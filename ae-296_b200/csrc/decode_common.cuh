@@ -7,7 +7,7 @@
 namespace b200lora {
 
 // ---- append ---------------------------------------------------------------------------------
-cudaError_t launch_kv_append(const b200_append& a, const b200_kv_cache& c, int dtype, bool vectors, cudaStream_t s);
+cudaError_t launch_kv_append(const b200_append& a, const b200_kv_cache& c, int dtype, bool vectors, int n_sm, cudaStream_t s);
 
 // ---- attention ------------------------------------------------------------------------------
 // The work of a call is cut into units: one unit is kKeys keys of one row tile (at most kRows query rows that read

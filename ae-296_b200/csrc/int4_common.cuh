@@ -13,7 +13,7 @@ constexpr int kInt4MaxSplit = 8;              // blocks of a cluster that share 
 struct Int4Params {
     alignas(64) CUtensorMap codes, x;
     b200_int4 a;
-    int y_f32, split, x_panels;
+    int y_f32, split, x_panels, early;       // early: a successor's blocks may come at once
 };
 
 namespace {
@@ -149,9 +149,9 @@ inline int int4_split(long long tiles, int stages, int at_once) {
 }
 
 // launch of a cluster of p.split blocks along y
-template <typename K>
-inline cudaError_t launch_int4_kernel(K kernel, const Int4Params& p, dim3 grid, int threads, size_t smem, cudaStream_t s) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+template <auto KERNEL>
+inline cudaError_t launch_int4_kernel(const Int4Params& p, dim3 grid, int threads, size_t smem, cudaStream_t s) {
+    const cudaError_t e = allow_smem<KERNEL>((int)smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
@@ -165,7 +165,7 @@ inline cudaError_t launch_int4_kernel(K kernel, const Int4Params& p, dim3 grid, 
     attr[1].val.clusterDim.x = 1; attr[1].val.clusterDim.y = (unsigned)p.split; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.split > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    return cudaLaunchKernelEx(&cfg, KERNEL, p);
 }
 
 // Codes as 16-bit numbers [n_out, n_in / 4], boxes of 128 bytes by 128 rows.  x as panels of 64 columns where they divide

@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
         sh.err = 0u;
     }
     pdl_wait_prior();
+    if (p.early && tid == 0) pdl_launch_dependents();
     __syncthreads();
     if (tid == 0)
         for (int s = 0; s < kStages && s < n; ++s) request(s);
@@ -174,9 +175,9 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(sh.empty[slot]));
     }
-    // Only now may a successor's blocks come: earlier they would take places on the SMs that have fewer blocks of this grid, and
-    // all SMs would have to wait for those (8192 columns, 32000 rows: 61 us instead of 44 us, back to back).
-    if (tid == 0) pdl_launch_dependents();
+    // A grid of more blocks than SMs lets a successor's come only now: earlier they would take places on the SMs that have fewer
+    // blocks of this grid, and all SMs would have to wait for those (8192 columns, 32000 rows: 61 us instead of 44 us, back to back).
+    if (!p.early && tid == 0) pdl_launch_dependents();
     // ---- sums to shared memory, where the codes were
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem);
@@ -193,8 +194,9 @@ cudaError_t launch_group(const b200_int4& a, int y_f32, int n_sm, cudaStream_t s
     p.a = a; p.y_f32 = y_f32;
     if (!encode_int4(p, kTokens, kStageK / 64)) return cudaErrorInvalidValue;
     const int tiles = (a.n_out + kRows - 1) / kRows, stages = (a.n_in + kStageK - 1) / kStageK;
-    p.split = int4_split(tiles, stages, n_sm);
-    return launch_int4_kernel(int4_few_kernel<T, G>, p, dim3((unsigned)tiles, (unsigned)p.split), kThreads, Few<G>::kBytes + sizeof(FewShared) + 1024, s);
+    p.split = int4_split(tiles, stages, 2 * n_sm);
+    p.early = p.split > 1;
+    return launch_int4_kernel<int4_few_kernel<T, G>>(p, dim3((unsigned)tiles, (unsigned)p.split), kThreads, Few<G>::kBytes + sizeof(FewShared) + 1024, s);
 }
 template <typename T>
 cudaError_t launch_typed(const b200_int4& a, int y_f32, int n_sm, cudaStream_t s) {

@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
     tc_fence_after();
     const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&sh.tmem);
     pdl_wait_prior();
+    if (p.early && tid == 0) pdl_launch_dependents();
 
     float acc[N];                                             // of the summing threads
 #pragma unroll
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
             if (lane == 0) mbar_arrive(bar(sh.d_empty[b % S::kSums]));
         }
     }
-    if (tid == 0) pdl_launch_dependents();                    // late, as in int4_few.cu
+    if (!p.early && tid == 0) pdl_launch_dependents();                    // late, as in int4_few.cu
     // ---- sums to shared memory, where x was (all multiplications are complete: they were summed)
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem + S::kStages * kCodeStage);
@@ -272,7 +273,8 @@ cudaError_t launch_tokens(const b200_int4& a, int y_f32, int n_sm, cudaStream_t 
     if (!encode_int4(p, N, 2)) return cudaErrorInvalidValue;
     const int tiles = (a.n_out + kRows - 1) / kRows, stages = (a.n_in + kStageK - 1) / kStageK, blocks = (a.n_tokens + N - 1) / N;
     p.split = int4_split((long long)tiles * blocks, stages, n_sm);
-    return launch_int4_kernel(int4_kernel<T, G, N>, p, dim3((unsigned)tiles, (unsigned)p.split, (unsigned)blocks), Shape<G, N>::kThreads,
+    p.early = (long long)tiles * blocks * p.split <= n_sm;
+    return launch_int4_kernel<int4_kernel<T, G, N>>(p, dim3((unsigned)tiles, (unsigned)p.split, (unsigned)blocks), Shape<G, N>::kThreads,
                               Shape<G, N>::kBytes + sizeof(Int4Shared) + 1024, s);
 }
 template <typename T, int G>

@@ -11,8 +11,11 @@ namespace b200lora {
 namespace {
 
 constexpr int kAppendThreads = 256;
+constexpr int kBlocksPerSm = 16;
 
+struct Side { const void *x, *dx; void* y; long long x_row, x_head, dx_row, dx_head, y_head; };     // q, k or v
 struct AppendParams {
+    Side side[3];
     b200_append a;
     b200_kv_cache c;
     int units;             // of a head
@@ -27,10 +30,15 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// VEC elements as they are in memory
+template <typename T, int VEC> struct Raw { uint4 v; };
+template <typename T> struct Raw<T, 1> { T v; };
 template <typename T, int VEC>
-__device__ __forceinline__ void load(const T* p, float (&f)[VEC]) {
-    if constexpr (VEC == 8) Cvt<T>::unpack8(*reinterpret_cast<const uint4*>(p), f);
-    else f[0] = to_f<T>(*p);
+__device__ __forceinline__ Raw<T, VEC> fetch(const T* p) { return *reinterpret_cast<const Raw<T, VEC>*>(p); }
+template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Raw<T, VEC>& r, float (&f)[VEC]) {
+    if constexpr (VEC == 8) Cvt<T>::unpack8(r.v, f);
+    else f[0] = to_f<T>(r.v);
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
@@ -43,7 +51,7 @@ __device__ __forceinline__ void store(T* p, const float (&f)[VEC]) {
 }
 template <typename T, int VEC>
 __device__ __forceinline__ void load_table(const void* tab, int f32, long long at, float (&f)[VEC]) {
-    if (!f32) { load<T, VEC>(static_cast<const T*>(tab) + at, f); return; }
+    if (!f32) { unpack<T, VEC>(fetch<T, VEC>(static_cast<const T*>(tab) + at), f); return; }
     const float* p = static_cast<const float*>(tab) + at;
     if constexpr (VEC == 8) {
         const float4 lo = reinterpret_cast<const float4*>(p)[0], hi = reinterpret_cast<const float4*>(p)[1];
@@ -55,7 +63,7 @@ __device__ __forceinline__ long long index_at(const void* p, int i64, long long 
 }
 
 template <typename T, int VEC>
-__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) kv_append_kernel(const __grid_constant__ AppendParams p) {
     pdl_wait_prior();
     if (threadIdx.x == 0) pdl_launch_dependents();
     const b200_append& a = p.a;
@@ -64,8 +72,35 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     const long long t = (long long)blockIdx.x * p.tokens_per_block + sub;
     if (sub >= p.tokens_per_block || t >= a.n_tokens) return;
     const long long slot = index_at(a.slots, a.slots_are_i64, t);
-    if (slot < 0) return;
     const long long pos = index_at(a.positions, a.positions_are_i64, t);
+    const int n_q = a.n_heads, n_kv = p.c.n_kv_heads, n_all = n_q + 2 * n_kv;
+    const bool turned = unit * 2 * VEC < a.rotary_dim;
+    const bool halves = turned && !a.interleaved;
+    const int lo = halves ? unit * VEC : unit * 2 * VEC, hi = halves ? lo + a.rotary_dim / 2 : lo + VEC;
+    const int vlo = unit * 2 * VEC, vhi = vlo + VEC;      // of v, which is not turned
+    const int step = gridDim.y * p.heads_per_pass;
+    Raw<T, VEC> x0, x1, d0, d1;
+    int which = 0, at0 = 0, at1 = 0;
+    long long head = 0;
+    auto ask = [&](int h) {
+        which = h < n_q ? 0 : h < n_q + n_kv ? 1 : 2;
+        head = h - (which == 0 ? 0 : which == 1 ? n_q : n_q + n_kv);
+        at0 = which == 2 ? vlo : lo;
+        at1 = which == 2 ? vhi : hi;
+        const Side& s = p.side[which];
+        const T* from = static_cast<const T*>(s.x) + t * s.x_row + head * s.x_head;
+        x0 = fetch<T, VEC>(from + at0);
+        x1 = fetch<T, VEC>(from + at1);
+        if (s.dx) {
+            const T* more = static_cast<const T*>(s.dx) + t * s.dx_row + head * s.dx_head;
+            d0 = fetch<T, VEC>(more + at0);
+            d1 = fetch<T, VEC>(more + at1);
+        }
+    };
+    int h = (int)blockIdx.y * p.heads_per_pass + lane_head - sub * p.heads_per_pass;
+    if (h >= n_all) return;
+    ask(h);                                               // (also for a row that is left out: q, k and v have it)
+    if (slot < 0) return;
     const long long page = slot / p.c.page_size;
     const int bad = (page >= p.c.n_pages ? B200_DECODE_BAD_SLOT : 0) | (pos < 0 || pos >= a.n_positions ? B200_DECODE_BAD_POSITION : 0);
     if (bad) {
@@ -73,73 +108,69 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
         return;
     }
     const long long place = page * p.c.page_stride + (slot - page * p.c.page_size) * p.c.token_stride;
-    const int n_q = a.n_heads, n_kv = p.c.n_kv_heads, n_all = n_q + 2 * n_kv;
-    const bool turned = unit * 2 * VEC < a.rotary_dim;
-    const bool halves = turned && !a.interleaved;
-    const int lo = halves ? unit * VEC : unit * 2 * VEC, hi = halves ? lo + a.rotary_dim / 2 : lo + VEC;
-    const int vlo = unit * 2 * VEC, vhi = vlo + VEC;      // of v, which is not turned
     float cs[VEC], sn[VEC];
     if (turned) {
         load_table<T, VEC>(a.cos, a.tables_are_f32, pos * a.table_row + unit * VEC, cs);
         load_table<T, VEC>(a.sin, a.tables_are_f32, pos * a.table_row + unit * VEC, sn);
     }
-    for (int h = (int)blockIdx.y * p.heads_per_pass + lane_head - sub * p.heads_per_pass; h < n_all; h += gridDim.y * p.heads_per_pass) {
-        const bool is_q = h < n_q, is_v = h >= n_q + n_kv;
-        const int hh = is_q ? h : is_v ? h - n_q - n_kv : h - n_q;
-        const T* x = static_cast<const T*>(is_q ? a.q : is_v ? a.v : a.k) +
-                     t * (is_q ? a.q_row : is_v ? a.v_row : a.k_row) + hh * (is_q ? a.q_head : is_v ? a.v_head : a.k_head);
-        const T* dx = static_cast<const T*>(is_q ? a.dq : is_v ? a.dv : a.dk);
-        T* y = is_q ? static_cast<T*>(a.q_out) + t * a.q_out_row + hh * a.q_out_head
-                    : static_cast<T*>(is_v ? p.c.v : p.c.k) + place + hh * p.c.head_stride;
-        const int at0 = is_v ? vlo : lo, at1 = is_v ? vhi : hi;
+    while (true) {
+        const Side& s = p.side[which];
         float f0[VEC], f1[VEC];
-        load<T, VEC>(x + at0, f0);
-        load<T, VEC>(x + at1, f1);
-        if (dx) {
-            dx += t * (is_q ? a.dq_row : is_v ? a.dv_row : a.dk_row) + hh * (is_q ? a.dq_head : is_v ? a.dv_head : a.dk_head);
-            float d0[VEC], d1[VEC];
-            load<T, VEC>(dx + at0, d0);
-            load<T, VEC>(dx + at1, d1);
+        unpack<T, VEC>(x0, f0);
+        unpack<T, VEC>(x1, f1);
+        if (s.dx) {
+            float e0[VEC], e1[VEC];
+            unpack<T, VEC>(d0, e0);
+            unpack<T, VEC>(d1, e1);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) { f0[i] += d0[i]; f1[i] += d1[i]; }
+            for (int k = 0; k < VEC; ++k) { f0[k] += e0[k]; f1[k] += e1[k]; }
         }
-        if (turned && !is_v) {
-            auto turn = [](float& x0, float& x1, float c, float s) {
-                const float y0 = x0 * c - x1 * s, y1 = x1 * c + x0 * s;
-                x0 = y0; x1 = y1;
+        if (turned && which < 2) {
+            auto turn = [](float& u, float& v, float c, float s) {
+                const float y0 = u * c - v * s, y1 = v * c + u * s;
+                u = y0; v = y1;
             };
             if (a.interleaved) {
                 if constexpr (VEC == 1) turn(f0[0], f1[0], cs[0], sn[0]);
                 else {
 #pragma unroll
-                    for (int i = 0; i < VEC / 2; ++i) {
-                        turn(f0[2 * i], f0[2 * i + 1], cs[i], sn[i]);
-                        turn(f1[2 * i], f1[2 * i + 1], cs[VEC / 2 + i], sn[VEC / 2 + i]);
+                    for (int k = 0; k < VEC / 2; ++k) {
+                        turn(f0[2 * k], f0[2 * k + 1], cs[k], sn[k]);
+                        turn(f1[2 * k], f1[2 * k + 1], cs[VEC / 2 + k], sn[VEC / 2 + k]);
                     }
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) turn(f0[i], f1[i], cs[i], sn[i]);
+                for (int k = 0; k < VEC; ++k) turn(f0[k], f1[k], cs[k], sn[k]);
             }
         }
+        T* y = static_cast<T*>(s.y) + (which == 0 ? t * a.q_out_row : place) + head * s.y_head;
         store<T, VEC>(y + at0, f0);
         store<T, VEC>(y + at1, f1);
+        h += step;
+        if (h >= n_all) return;
+        ask(h);
     }
 }
 
 }  // namespace
 
-cudaError_t launch_kv_append(const b200_append& a, const b200_kv_cache& c, int dtype, bool vectors, cudaStream_t s) {
+cudaError_t launch_kv_append(const b200_append& a, const b200_kv_cache& c, int dtype, bool vectors, int n_sm, cudaStream_t s) {
     AppendParams p;
     p.a = a; p.c = c;
+    p.side[0] = {a.q, a.dq, a.q_out, a.q_row, a.q_head, a.dq_row, a.dq_head, a.q_out_head};
+    p.side[1] = {a.k, a.dk, c.k, a.k_row, a.k_head, a.dk_row, a.dk_head, c.head_stride};
+    p.side[2] = {a.v, a.dv, c.v, a.v_row, a.v_head, a.dv_row, a.dv_head, c.head_stride};
     p.units = c.head_dim / (vectors ? 16 : 2);
     const int lanes = kAppendThreads / p.units, heads = a.n_heads + 2 * c.n_kv_heads;
     p.heads_per_pass = lanes < heads ? lanes : heads;
     p.tokens_per_block = lanes / p.heads_per_pass;
     const unsigned blocks = (unsigned)((a.n_tokens + (long long)p.tokens_per_block - 1) / p.tokens_per_block);
-    // few tokens: one pass per block, so that all heads move at once
+    // Few tokens: one pass per block, so that all heads move at once.  Many: a block keeps a token's sines and its address for as
+    // many heads as leave about kBlocksPerSm blocks for every SM.
     const int passes = (heads + p.heads_per_pass - 1) / p.heads_per_pass;
-    const dim3 grid(blocks, (unsigned)passes);
+    const unsigned want = (unsigned)(kBlocksPerSm * n_sm) / blocks + 1;
+    const dim3 grid(blocks, want < (unsigned)passes ? want : (unsigned)passes);
     if (dtype == B200_LORA_F16)
         return launch_pdl(vectors ? kv_append_kernel<__half, 8> : kv_append_kernel<__half, 1>, grid, kAppendThreads, 0, s, p);
     return launch_pdl(vectors ? kv_append_kernel<__nv_bfloat16, 8> : kv_append_kernel<__nv_bfloat16, 1>, grid, kAppendThreads, 0, s, p);

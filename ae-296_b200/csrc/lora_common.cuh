@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 #include <utility>
 
@@ -308,6 +309,18 @@ int cuda_fail(cudaError_t e);             // keeps the error's text for b200_lor
 int sm_count();                           // of the current device
 bool encode_map(CUtensorMap* out, const void* base, std::initializer_list<uint64_t> extents, std::initializer_list<uint64_t> strides,
                 std::initializer_list<uint32_t> box);
+
+// Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device; KERNEL distinguishes the flags.
+template <auto KERNEL>
+inline cudaError_t allow_smem(int bytes) {
+    static std::atomic<int> allowed[64];
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev >= 0 && dev < 64 && allowed[dev].load(std::memory_order_relaxed) >= bytes)) return e;
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) allowed[dev].store(bytes, std::memory_order_relaxed);
+    return e;
+}
 
 // ---- launchers implemented by the kernel files ---------------------------------------------
 struct PlanAdapters {          // what the plan bakes into its unit records
