@@ -67,7 +67,7 @@ __device__ __forceinline__ int page_at(const AttnParams& p, const PageWalk& w, i
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_constant__ AttnParams p) {
-    extern __shared__ __align__(1024) unsigned char smem[];
+    extern __shared__ __align__(128) unsigned char smem[];
     using R = Ring<D>;
     int* su = reinterpret_cast<int*>(smem + R::kBytes);      // units before each entity
     int* st = su + p.a.n_groups + p.a.n_requests + 1;        // tiles before each group
@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
     pdl_launch_dependents();
 }
 
+constexpr int kJoin = 4;
 // One warp per query row: the row's parts of its group's item and of its own item, weighted by 2^(m_i - max m).
 template <typename T, int D>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnParams p) {
@@ -283,42 +284,9 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     const int workers = (int)min((long long)p.workers, total);
 
     constexpr int V = D / 32;
-    float acc[V], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int k = 0; k < V; ++k) acc[k] = 0.f;
-    // parts [w0, w1] at rows slot + w * pitch
-    auto add = [&](size_t slot, int pitch, int w0, int w1) {
-        for (int base = w0; base <= w1; base += 32) {
-            const bool there = base + lane <= w1;
-            const float2 ml = there ? __ldcg(p.part_ml + slot + (size_t)(base + lane) * pitch) : make_float2(-INFINITY, 0.f);
-            float top = ml.x;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const float to = fmaxf(m, top), ref = to == -INFINITY ? 0.f : to;
-            const float old = exp2f(m - ref), w = exp2f(ml.x - ref);
-            m = to;
-            float sum = w * ml.y;
-#pragma unroll
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            l = l * old + sum;
-#pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] *= old;
-            const int n = min(32, w1 - base + 1);
-#pragma unroll 4
-            for (int j = 0; j < n; ++j) {
-                const float wj = __shfl_sync(0xffffffffu, w, j);
-                if (wj == 0.f) continue;                       // a part without keys may have no sums either
-                const float* src = p.part + (slot + (size_t)(base + j) * pitch) * D + lane * V;
-                if constexpr (V == 4) {
-                    const float4 f = __ldcg(reinterpret_cast<const float4*>(src));
-                    acc[0] += wj * f.x; acc[1] += wj * f.y; acc[2] += wj * f.z; acc[3] += wj * f.w;
-                } else {
-                    const float2 f = __ldcg(reinterpret_cast<const float2*>(src));
-                    acc[0] += wj * f.x; acc[1] += wj * f.y;
-                }
-            }
-        }
-    };
+    // The row's parts: those of its group's item (a wide tile of one stream's rows has a second part for each), then of its own.  Part
+    // i of a run lies at row first + i * pitch.
+    struct Run { size_t first; int pitch, n; } run[3] = {{0, 0, 0}, {0, 0, 0}, {0, 0, 0}};
     if (n_g > 0 && p.tiles[0] >= 0) {                          // starts ascend
         int lo = -1, hi = n_g;                                 // last group that starts at or before b
         while (hi - lo > 1) {
@@ -337,13 +305,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
                 const size_t item = (size_t)n_kv * before[lo] + (size_t)h * tiles + tile;
                 const long long sum = wide ? (long long)p.wide_units[n_g] * n_kv : total;
                 const int w = wide ? (int)min((long long)p.wide_workers, sum) : workers;
-                const int w0 = worker_of_unit(sum, u0, w), w1 = worker_of_unit(sum, u0 + chunks - 1, w);
-                if (!wide) add(item * kAttnRows + (r - tile * kAttnRows), kAttnRows, w0, w1);
+                const int w0 = worker_of_unit(sum, u0, w), n = worker_of_unit(sum, u0 + chunks - 1, w) - w0 + 1;
+                if (!wide) run[0] = {(item + w0) * kAttnRows + (r - tile * kAttnRows), kAttnRows, n};
                 else {
-                    const size_t row = attn_group_rows(p) + attn_request_rows(p) + item * kWideRows + (r - tile * kWideRows);
-                    add(row, kWideRows, w0, w1);
-                    // a tile of one stream's rows: the second stream's parts, over the other keys, lie behind them
-                    if (n_rows - tile * kWideRows <= kWideRows / 2) add(row + kWideRows / 2, kWideRows, w0, w1);
+                    run[0] = {attn_group_rows(p) + attn_request_rows(p) + (item + w0) * kWideRows + (r - tile * kWideRows), kWideRows, n};
+                    if (n_rows - tile * kWideRows <= kWideRows / 2) run[1] = {run[0].first + kWideRows / 2, kWideRows, n};
                 }
             }
         }
@@ -353,8 +319,58 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
         const int chunks = all / p.req_tiles, tile = i / kAttnRows;
         const long long u0 = (long long)n_kv * p.units[e] + (long long)h * all + (long long)tile * chunks;
         const size_t item = ((size_t)b * n_kv + h) * p.req_tiles + tile;
-        add(attn_group_rows(p) + item * p.req_rows + (i - tile * kAttnRows), p.req_rows, worker_of_unit(total, u0, workers),
-            worker_of_unit(total, u0 + chunks - 1, workers));
+        const int w0 = worker_of_unit(total, u0, workers);
+        run[2] = {attn_group_rows(p) + (item + w0) * p.req_rows + (i - tile * kAttnRows), p.req_rows, worker_of_unit(total, u0 + chunks - 1, workers) - w0 + 1};
+    }
+    auto part_at = [&](int k) {
+        if (k < run[0].n) return run[0].first + (size_t)k * run[0].pitch;
+        k -= run[0].n;
+        if (k < run[1].n) return run[1].first + (size_t)k * run[1].pitch;
+        return run[2].first + (size_t)(k - run[1].n) * run[2].pitch;
+    };
+    float acc[V], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] = 0.f;
+    const int parts = run[0].n + run[1].n + run[2].n;
+    for (int base = 0; base < parts; base += 32) {
+        // a part a lane: maxima and sums
+        const int n = min(32, parts - base);
+        const size_t at = part_at(base + min(lane, n - 1));
+        const float2 ml = lane < n ? __ldcg(p.part_ml + at) : make_float2(-INFINITY, 0.f);
+        float top = ml.x;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float to = fmaxf(m, top), ref = to == -INFINITY ? 0.f : to;
+        const float old = exp2f(m - ref), w = exp2f(ml.x - ref);
+        m = to;
+        float sum = w * ml.y;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        l = l * old + sum;
+#pragma unroll
+        for (int k = 0; k < V; ++k) acc[k] *= old;
+        for (int j = 0; j < n; j += kJoin) {
+            // the rows of kJoin parts are asked for together; those of a part without keys may be anything
+            float f[kJoin][V];
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                const float* src = p.part + __shfl_sync(0xffffffffu, at, min(j + k, n - 1)) * D + lane * V;
+                if constexpr (V == 4) {
+                    const float4 g = __ldcg(reinterpret_cast<const float4*>(src));
+                    f[k][0] = g.x; f[k][1] = g.y; f[k][2] = g.z; f[k][3] = g.w;
+                } else {
+                    const float2 g = __ldcg(reinterpret_cast<const float2*>(src));
+                    f[k][0] = g.x; f[k][1] = g.y;
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kJoin; ++k) {
+                const float wk = __shfl_sync(0xffffffffu, w, min(j + k, 31));
+                if (j + k < n && wk != 0.f)
+#pragma unroll
+                    for (int c = 0; c < V; ++c) acc[c] += wk * f[k][c];
+            }
+        }
     }
     const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;  // no key: zeros; NaN stays NaN
     T* out = static_cast<T*>(p.a.out) + (long long)b * p.a.out_row + (long long)hq * p.a.out_head + lane * V;

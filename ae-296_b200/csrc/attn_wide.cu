@@ -100,19 +100,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     unsigned* err = &sh.err;
 
     pdl_wait_prior();
-    if (tid == 0) {
-        pdl_launch_dependents();
-        for (int i = 0; i < RING; ++i) { mbar_init(bar(sh.full[i]), kCopyThreads); mbar_init(bar(sh.empty[i]), 1); }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(bar(sh.q_ready[s]), kStreamRows);
-            mbar_init(bar(sh.p_ready[s]), kStreamRows);
-            mbar_init(bar(sh.s_full[s]), 1);
-            mbar_init(bar(sh.o_full[s]), 1);
+    if (tid == 0) pdl_launch_dependents();
+    if (tid < kMaxRing) {
+        if (tid < RING) { mbar_init(bar(sh.full[tid]), kCopyThreads); mbar_init(bar(sh.empty[tid]), 1); }
+        if (tid < 2) {
+            mbar_init(bar(sh.q_ready[tid]), kStreamRows);
+            mbar_init(bar(sh.p_ready[tid]), kStreamRows);
+            mbar_init(bar(sh.s_full[tid]), 1);
+            mbar_init(bar(sh.o_full[tid]), 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        sh.err = 0u;
-        sh.bad = 0;
     }
+    if (tid == 0) { sh.err = 0u; sh.bad = 0; }
     __syncthreads();
     const int n_g = p.a.n_groups, n_kv = p.c.n_kv_heads;
     const bool usable = scan_units<kThreads>(n_g, n_g, su, st, sh.warp_sum, &sh.bad, [&](int e, bool ok, int& bad) {
@@ -170,6 +169,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             int b = block_at(0, is_v);
             read_table(b);
             for (int i = 0; i < 2 * t.n; ++i, ++n) {
+                if (u == u_first && i == 1) {    // the first multiplication needs the queries and one block: the others wait for those
+                    for (int q = 0; q < 2; ++q)
+                        if (t.dual || q < t.n) mbar_wait(bar(sh.q_ready[q]), 0, err, 7);
+                }
                 const int slot = n % RING;
                 mbar_wait(bar(sh.empty[slot]), ((n / RING) & 1) ^ 1, err, 1);
                 __syncwarp();
@@ -289,6 +292,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
         const int s = warp >> 2, row = tid & 127;
         const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
         const unsigned s_tm = tmem + lanes + s * 128, o_tm = tmem + lanes + 256 + s * 128;
+        auto stream_sync = [&]() {
+            if (s == 0) asm volatile("bar.sync 1, %0;" ::"n"(kStreamRows) : "memory");
+            else asm volatile("bar.sync 2, %0;" ::"n"(kStreamRows) : "memory");
+        };
         // scores are compared as they come from the multiplication: a negative scale goes into the queries' signs
         const unsigned flip = p.scale_log2 < 0.f ? 0x80008000u : 0u;
         const float scale = fabsf(p.scale_log2);
@@ -301,15 +308,25 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             const int step = t.dual ? 1 : 2, b_first = t.dual ? 0 : s;
             // ---- queries to shared memory (the stream's last multiplication that reads them is complete)
             if (b_first < t.n) {
-                const int ra = t.tile * kWideRows + (live ? r_in : 0);
-                const T* q = static_cast<const T*>(p.a.q) + (long long)(t.first + ra / p.per) * p.a.q_row + (long long)(t.h * p.per + ra % p.per) * p.a.q_head;
                 const unsigned qa = smem_u32(smem) + s * W::kQ;
+                constexpr int kPieces = D / 8, kBatch = 8;
+                const int c = row % kPieces;
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    uint4 v = *reinterpret_cast<const uint4*>(q + c * 8);
-                    if (!live) v = make_uint4(0u, 0u, 0u, 0u);
-                    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};"
-                                 ::"r"(swizzled(qa, row, c)), "r"(v.x ^ flip), "r"(v.y ^ flip), "r"(v.z ^ flip), "r"(v.w ^ flip) : "memory");
+                for (int i0 = 0; i0 < kPieces; i0 += kBatch) {
+                    uint4 v[kBatch];
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i) {           // neighbouring lanes read neighbouring pieces of a row
+                        const int r = ((i0 + i) * kStreamRows + row) / kPieces, in_tile = t.dual ? s * kStreamRows + r : r;
+                        v[i] = make_uint4(flip, flip, flip, flip);
+                        if (in_tile < t.rows) {
+                            const int ra = t.tile * kWideRows + in_tile, request = ra / p.per;
+                            v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + (long long)(t.first + request) * p.a.q_row +
+                                                                    (long long)(t.h * p.per + ra - request * p.per) * p.a.q_head + c * 8);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < kBatch; ++i)
+                        sts16(swizzled(qa, ((i0 + i) * kStreamRows + row) / kPieces, c), v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
                 }
                 fence_async_proxy();
                 mbar_arrive(bar(sh.q_ready[s]));
@@ -402,20 +419,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                 ++outs;
                 __syncwarp();
                 tc_fence_after();
-                if (warp_live) {
-                    float* dst = p.part + out_row * D;
+                // Rows go out through the place of the queries, half a row of each at a time: by themselves the lanes' rows lie D words
+                // apart, and every 16 bytes would be a transfer of their own.
+                const unsigned at = smem_u32(smem) + s * W::kQ;
+                constexpr int kPieces = D / 8;                   // of 16 bytes, of half a row
+                const int c_out = row % kPieces;
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        unsigned o[32];
-                        tc_ld32(o_tm + c * 32, o);
-                        tc_wait_ld();
-                        if (live) {
+                for (int turn = 0; turn < 2; ++turn) {
+                    if (warp_live) {
+#pragma unroll
+                        for (int c = 0; c < D / 64; ++c) {
+                            unsigned o[32];
+                            tc_ld32(o_tm + turn * (D / 2) + c * 32, o);
+                            tc_wait_ld();
 #pragma unroll
                             for (int j = 0; j < 8; ++j)
-                                reinterpret_cast<uint4*>(dst + c * 32)[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                                sts16(at + row * (D * 2) + (((c * 8 + j) ^ (row & 7)) << 4), o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
                         }
+                        tc_fence_before();
                     }
-                    tc_fence_before();
+                    stream_sync();
+#pragma unroll 4
+                    for (int i = 0; i < kPieces; ++i) {
+                        const int r = (i * kStreamRows + row) / kPieces, in_tile = t.dual ? s * kStreamRows + r : r;
+                        unsigned w[4];
+                        lds16(at + r * (D * 2) + ((c_out ^ (r & 7)) << 4), w);
+                        if (in_tile < t.rows)
+                            reinterpret_cast<uint4*>(p.part + (t.slot + s * kStreamRows + r) * D + turn * (D / 2))[c_out] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    stream_sync();
                 }
                 if (live) p.part_ml[out_row] = make_float2(m == -INFINITY ? m : m - kLift, l);
             } else if (live) p.part_ml[out_row] = make_float2(-INFINITY, 0.f);

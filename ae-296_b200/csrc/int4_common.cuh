@@ -52,12 +52,6 @@ __device__ __forceinline__ float4 remote_f32x4(unsigned addr, unsigned rank) {
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
     return v;
 }
-__device__ __forceinline__ void tc_ld16(unsigned taddr, unsigned (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-                   "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr));
-}
 // Eight columns, in order, of a word of codes; o: what takes the zero point away (zero_offset).  Columns 2 i are the low four bits of
 // byte i and become the low halves of the pairs; columns 2 i + 1 stay 16 times as large in the high ones, and the multiplier
 // differs instead.  The zero bytes between are the sign, eight times, of a byte that is below 128.
@@ -81,9 +75,6 @@ __device__ __forceinline__ bool mbar_passed(unsigned bar, unsigned parity) {
     asm volatile("{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok != 0;
-}
-__device__ __forceinline__ void lds16(unsigned addr, unsigned (&v)[4]) {
-    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void tensor_g2s_3d(unsigned dst, const void* map, int x, int y, int z, unsigned bar) {
