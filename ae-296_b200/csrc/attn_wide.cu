@@ -19,7 +19,7 @@
 // Warps 0..3 and 4..7: the streams.  Warp 8: one thread issues the multiplications.  Warps 9..11 bring keys and values
 // into a ring of blocks by asynchronous 16-byte copies in the 128-byte swizzled layout the multiplications read, page
 // by page, whatever the page size, with zeros in place of keys behind the prefix or in pages that do not exist.
-// Every wait is bounded: on expiry the block's error word is set, control flow stays as it is and the kernel ends.
+// Every wait is bounded: on expiry control flow stays as it is, and the outputs become NaN.
 #include <type_traits>
 
 #include "attn_common.cuh"
@@ -102,7 +102,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     pdl_wait_prior();
     if (tid == 0) pdl_launch_dependents();
     if (tid < kMaxRing) {
-        if (tid < RING) { mbar_init(bar(sh.full[tid]), kCopyThreads); mbar_init(bar(sh.empty[tid]), 1); }
+        if (tid < RING) { mbar_init(bar(sh.full[tid]), kCopyThreads + kCopyWarps); mbar_init(bar(sh.empty[tid]), 1); }
         if (tid < 2) {
             mbar_init(bar(sh.q_ready[tid]), kStreamRows);
             mbar_init(bar(sh.p_ready[tid]), kStreamRows);
@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                     if (g < kGroups) cp_async16(swizzled(dst, row, piece), base + max(from, 0ll), from >= 0);
                 }
                 arrive_when_copied(bar(sh.full[slot]));
+                if (lane == 0) mbar_arrive(bar(sh.full[slot]));  // (for what it wrote by itself: the missing keys)
                 b = next;
                 is_v = next_v;
             }
@@ -458,7 +459,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     if (warp == 8) tmem_dealloc(tmem);
-    if (tid == 0 && sh.err && p.a.status) atomicOr(p.a.status, B200_DECODE_TIMEOUT);
+    if (sh.err) {
+        if (tid == 0 && p.a.status) atomicOr(p.a.status, B200_DECODE_TIMEOUT);
+        for (long long u = u_first; u < u_end;) {             // the join makes NaN of these
+            const Part t = part_at(u);
+            if (tid < kWideRows) p.part_ml[t.slot + tid] = make_float2(INFINITY, __int_as_float(0x7fffffff));
+            u += t.n;
+        }
+    }
 }
 
 template <typename T, int D, int RING>

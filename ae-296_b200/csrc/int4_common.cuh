@@ -117,8 +117,8 @@ __device__ __forceinline__ void finish_sums(const Int4Params& p, const float* re
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (col + i >= a.n_out) break;
-            if (p.y_f32) static_cast<float*>(a.y)[to + i] = f[i] + g[i];
-            else static_cast<T*>(a.y)[to + i] = (T)(f[i] + g[i]);
+            if (p.y_f32) static_cast<float*>(a.y)[to + i] = fmaf(f[i], Codes<T>::kInverse, g[i]);
+            else static_cast<T*>(a.y)[to + i] = (T)fmaf(f[i], Codes<T>::kInverse, g[i]);
         }
     }
     if (p.split > 1) cluster_sync();                          // nobody leaves while its sums are read

@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
         uint2* to = factors + ((chunk & 1) * kRows + f_row) * F::kPitch + f_first;
 #pragma unroll
         for (int i = 0; i < kHalf; ++i)
-            to[i] = make_uint2(__float_as_uint(from_bits<T>((unsigned short)((i < 2 ? sc.x : sc.y) >> (16 * (i & 1)))) * Codes<T>::kInverse),
+            to[i] = make_uint2(__float_as_uint(from_bits<T>((unsigned short)((i < 2 ? sc.x : sc.y) >> (16 * (i & 1))))),
                                zero_offset<T>(ze >> (8 * i) & 15u));
     };
     load_factors(0);

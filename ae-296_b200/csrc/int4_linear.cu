@@ -6,8 +6,8 @@
 // rounded before y.
 //
 // A code becomes a number without a magic constant: four bits zero-extended to 16 are a subnormal number, and one
-// multiply-add brings it to size and takes the zero point away (value c - z times a power of two that the scale
-// takes back).  A 32-bit word of eight codes costs two logic operations, four byte permutations and four multiply-adds.
+// multiply-add brings it to size and takes the zero point away (value c - z times a power of two that is taken
+// back from the whole sum, where it cannot make a large scale infinite).  A 32-bit word of eight codes costs two logic operations, four byte permutations and four multiply-adds.
 //
 // A block takes 128 rows and a part of the columns.  Two threads copy codes (128 rows by 256 columns a stage) and x (128
 // columns a block) by tensor copies; eight warps turn codes into 16-bit numbers, a lane per row, and store them to TMEM
@@ -30,7 +30,10 @@ constexpr int kStageK = 256, kBlockK = 128;
 constexpr int kCodeStage = kRows * kStageK / 2;               // 16 KB
 constexpr int kACols = kBlockK / 2;                           // TMEM columns of a block of numbers
 constexpr int kRedPitch = kRows + 4;                          // floats of a token's sums
-constexpr int kRing = 4;                                      // blocks of x, and barriers of finished blocks
+constexpr int kRing = 4;                                      // blocks of x
+// Barriers of finished blocks.  Half of the code warps may wait for block b - 3 while block b + 1, the other half's, ends: on the
+// same barrier that would be one round too many.
+constexpr int kDone = 8;
 
 // N: tokens of a block, G: columns of a group.  Few tokens: two blocks an SM share its memories.
 template <int G, int N> struct Shape {
@@ -43,7 +46,11 @@ template <int G, int N> struct Shape {
     static constexpr int kSumRoom = N == 16 ? (G == 32 ? 128 : 64) : 256;
     static constexpr int kSums = kSumRoom / kSumCols < 4 ? kSumRoom / kSumCols : 4;
     static constexpr int kNumbers = N == 16 ? (G == 32 ? 2 : 3) : 4;
-    static constexpr int kMmaWarps = N == 16 ? 2 : 4;
+    // A thread that waits for a barrier has waited for its last round too, or it could take the one before that for this one: the
+    // threads that issue divide the blocks of sums, of numbers (kReady barriers for those) and of x.
+    static constexpr int kMmaWarps = N == 16 || kSums == 2 ? 2 : 4;
+    static constexpr int kReady = kNumbers == 3 ? 6 : kNumbers;
+    static_assert(kSums % kMmaWarps == 0 && kReady % kMmaWarps == 0 && kReady % kNumbers == 0 && kRing % kMmaWarps == 0, "rounds in order");
     static constexpr int kThreads = (kMmaWarp + kMmaWarps) * 32;
     static constexpr int kUsed = kSums * kSumCols + kNumbers * kACols;
     static constexpr int kAlloc = kUsed <= 256 ? 256 : 512;
@@ -51,7 +58,7 @@ template <int G, int N> struct Shape {
     static_assert(N * kRedPitch * 4 <= kRing * kX, "the sums take x's place");
 };
 struct Int4Shared {
-    unsigned long long codes_full[8], codes_empty[8], x_full[kRing], done[kRing], a_full[4], d_empty[4];
+    unsigned long long codes_full[8], codes_empty[8], x_full[kRing], done[kDone], a_full[6], d_empty[4];
     unsigned tmem, err;
 };
 
@@ -71,14 +78,15 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
     auto bar = [](unsigned long long& b) { return smem_u32(&b); };
     unsigned* err = &sh.err;
     const unsigned codes_at = smem_u32(smem), x_at = codes_at + S::kStages * kCodeStage;
-    auto wait_done = [&](int b, unsigned code) { if (b >= 0) mbar_wait(bar(sh.done[b % kRing]), (b / kRing) & 1, err, code); };
+    auto wait_done = [&](int b, unsigned code) { if (b >= 0) mbar_wait(bar(sh.done[b % kDone]), (b / kDone) & 1, err, code); };
 
     if (warp == kCopyWarp && lane == 0) {
         // the codes are on their way to L2 while the predecessor ends (what it may still write, L2 sees too)
         for (int s = 0; s < S::kStages && s < n_stages; ++s) prefetch_tensor(&p.codes, (s0 + s) * (kStageK / 4), row0);
         for (int i = 0; i < S::kStages; ++i) { mbar_init(bar(sh.codes_full[i]), 1); mbar_init(bar(sh.codes_empty[i]), kCodeWarps); }
-        for (int i = 0; i < kRing; ++i) { mbar_init(bar(sh.x_full[i]), 1); mbar_init(bar(sh.done[i]), 1); }
-        for (int i = 0; i < S::kNumbers; ++i) mbar_init(bar(sh.a_full[i]), kCodeWarps / 2);
+        for (int i = 0; i < kRing; ++i) mbar_init(bar(sh.x_full[i]), 1);
+        for (int i = 0; i < kDone; ++i) mbar_init(bar(sh.done[i]), 1);
+        for (int i = 0; i < S::kReady; ++i) mbar_init(bar(sh.a_full[i]), kCodeWarps / 2);
         for (int i = 0; i < S::kSums; ++i) mbar_init(bar(sh.d_empty[i]), kSumWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.err = 0u;
@@ -131,14 +139,14 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
                 const int at = b % kRing, from = b % S::kNumbers, to = b % S::kSums;
                 mbar_wait(bar(sh.d_empty[to]), ((b / S::kSums) & 1) ^ 1, err, 3);
                 mbar_wait(bar(sh.x_full[at]), (b / kRing) & 1, err, 4);
-                mbar_wait(bar(sh.a_full[from]), (b / S::kNumbers) & 1, err, 5);
+                mbar_wait(bar(sh.a_full[b % S::kReady]), (b / S::kReady) & 1, err, 5);
                 tc_fence_after();
                 const unsigned xa = desc_low(x_at + at * S::kX, kRowsAreRows);
                 const unsigned w = tmem + S::kSums * S::kSumCols + from * kACols, d = tmem + to * S::kSumCols;
 #pragma unroll
                 for (int i = 0; i < kBlockK / 16; ++i)
                     mma_ts(d + (i * 16 / G) * N, w + i * 8, xa + (((i >> 2) * (S::kX / 2) + (i & 3) * 32) >> 4), idesc, i % (G / 16) != 0);
-                tc_commit(bar(sh.done[at]));
+                tc_commit(bar(sh.done[b % kDone]));
             }
         }
         __syncwarp();
@@ -199,7 +207,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar(sh.a_full[at]));
+            if (lane == 0) mbar_arrive(bar(sh.a_full[b % S::kReady]));
         }
     } else {
         // ================= sums: a thread per row =================
@@ -230,7 +238,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
         for (int b = 0; b < n_blocks; ++b) {
             float f[kPer];
 #pragma unroll
-            for (int g = 0; g < kPer; ++g) f[g] = from_bits<T>((unsigned short)((g < 2 ? sc[0].x : sc[0].y) >> (16 * (g & 1)))) * Codes<T>::kInverse;
+            for (int g = 0; g < kPer; ++g) f[g] = from_bits<T>((unsigned short)((g < 2 ? sc[0].x : sc[0].y) >> (16 * (g & 1))));
             sc[0] = sc[1]; sc[1] = sc[2]; sc[2] = sc[3];
             sc[3] = load_scales(b + 4);
             wait_done(b, 8);

@@ -22,7 +22,8 @@ from . import _lib
 from ._lib import check
 from .ops import _require_cuda
 
-BAD_SLOT, BAD_POSITION, BAD_PAGE, BAD_LENGTH, BAD_GROUPS = 1, 2, 4, 8, 16      # bits of a `status` word
+# bits of a `status` word; the last: a wait inside a kernel ran out, and the outputs concerned are NaN
+BAD_SLOT, BAD_POSITION, BAD_PAGE, BAD_LENGTH, BAD_GROUPS, TIMEOUT = 1, 2, 4, 8, 16, 32
 
 
 def _refuse(what: str, tests) -> None:
@@ -117,7 +118,7 @@ def prefix_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, 
     A request without any key gets zeros and ``lse`` -inf.  Whatever the cache holds behind the lengths, NaN included, has no
     influence.  Lengths and tables stay on the device; a page outside the cache is left out, a length outside its table is cut,
     group starts that do not ascend inside the batch leave all prefixes out; each sets its bit (``BAD_PAGE``, ``BAD_LENGTH``,
-    ``BAD_GROUPS``) in ``status`` (one int32 on the device, for the caller to clear and to read).  At most 4096 requests and 2048 groups."""
+    ``BAD_GROUPS``; ``TIMEOUT`` if a wait inside the kernel ran out) in ``status`` (one int32 on the device, for the caller to clear and to read).  At most 4096 requests and 2048 groups."""
     rc = _lib.host().prefix_attention(out, q, k_cache, v_cache, block_table, lens, prefix_table, prefix_lens, group_starts,
                                       q.shape[-1] ** -0.5 if scale is None else scale, lse, status)
     if rc > 0:

@@ -27,7 +27,7 @@ enum {
     B200_DECODE_BAD_LENGTH = 8,    /* attention: a negative length, or one longer than the row of the page table; it
                                       was taken as zero, or as the row's */
     B200_DECODE_BAD_GROUPS = 16,   /* attention: group starts that descend or lie outside the batch; no prefix was used */
-    B200_DECODE_TIMEOUT = 32     /* a bounded wait inside a kernel expired: the outputs cannot be used */
+    B200_DECODE_TIMEOUT = 32       /* attention: a bounded wait inside a kernel expired; the outputs concerned are NaN */
 };
 enum { B200_DECODE_MAX_REQUESTS = 4096, B200_DECODE_MAX_GROUPS = 2048 };
 
