@@ -8,13 +8,15 @@ random tensor (lightllm/models/lora_gpu.py:120,124).  Here they drive the op:
 * ``order_by_adapter``   the order in which a router should lay out the requests of a batch so that requests
                           of one adapter are neighbours (stable: arrival order is kept inside an adapter);
 * ``plan_for_requests``   the plan of a batch given exactly the three tensors the reference prepares;
+* ``prefix_groups``       the neighbours of one adapter in a decode batch, which can share the keys and values of a common
+                          prompt (:func:`ae296_b200.prefix_attention`);
 * ``delta_cost_us``       a cost estimate of the LoRA delta of a candidate batch for schedulers that compare
                           placements (the role ``cost_model.get_latency(n, rank_func(ranks))`` plays in
                           scheduler/scheduler/manager.py:52-98).
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -26,6 +28,20 @@ from .pool import AdapterPool
 def order_by_adapter(lora_ids: Sequence[int]) -> np.ndarray:
     """Indices that sort the requests by adapter id, arrival order kept inside one adapter."""
     return np.argsort(np.asarray(lora_ids, np.int64), kind="stable")
+
+
+def prefix_groups(lora_ids: Sequence[int]) -> Tuple[np.ndarray, np.ndarray]:
+    """``(group_starts int32 [G + 1], adapters int64 [G])`` of a decode batch: group ``g`` is the requests ``group_starts[g]`` to
+    ``group_starts[g + 1] - 1``, which all have adapter ``adapters[g]`` (its index, or the negative id of requests without one).
+
+    Deltas of k and v make a prompt's cache entries the adapter's own, so the requests that can share them are those of one
+    adapter.  In a batch laid out by :func:`order_by_adapter` every adapter is one group; in another order one that is split up
+    is several, each of which would read the prefix by itself.  A group without a common prompt gets a prefix length of 0."""
+    ids = np.asarray(lora_ids, np.int64)
+    if ids.ndim != 1:
+        raise ValueError("one id per request expected")
+    first = np.flatnonzero(np.concatenate([np.ones(min(1, len(ids)), bool), ids[1:] != ids[:-1]]))
+    return np.append(first, len(ids)).astype(np.int32), ids[first]
 
 
 def plan_for_requests(batch: LoraBatch, pool: AdapterPool, lora_ids: torch.Tensor, b_start_loc: torch.Tensor,

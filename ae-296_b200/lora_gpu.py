@@ -13,6 +13,7 @@ unchanged.  Differences, all on purpose:
   reproduces that op's fp16 rounding of the ``[B, L, r]`` intermediate;
 * adapter ids come from ``set_indices`` (the reference draws random ids once,
   lora_gpu.py:120, reading past its pool when ``batch_size < 32``);
+* ``append_one_layer`` does for a decode step what the layer code does with the three deltas next, in one launch;
 * no sockets, no swapper, no process exit on error: errors raise.
 """
 from __future__ import annotations
@@ -24,6 +25,7 @@ import torch
 import numpy as np
 
 from . import _lib
+from .decode import append_kv
 from .ops import LoraBatch, _adapters_struct, apply
 from .pool import AdapterPool
 
@@ -131,6 +133,20 @@ class Lora_GPU:
 
     def invoke_one_layer_v(self, x, layer_id, prefill=False):
         return self._invoke(2, x, layer_id, prefill)
+
+    def append_one_layer(self, x, layer_id, q_out, q, k, v, k_cache, v_cache, positions, slots, cos, sin,
+                         interleaved: bool = False, status: Optional[torch.Tensor] = None) -> None:
+        """A decode step's three deltas of ``x [bsz, H]`` and what the layer code does with them next
+        (lightllm/models/llama/layer_infer/transformer_layer_infer.py:108-111 and :160-170): added to the base
+        projections ``q``, ``k`` and ``v``, turned by position and written to the layer's cache in one further launch.
+        Arguments as in :func:`ae296_b200.append_kv`; q, k and v are ``[bsz, heads, D]`` with ``heads * D`` the width
+        of the up projections."""
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            if t.dim() != 3 or t.shape[0] != x.shape[0] or t.shape[1] * t.shape[2] != self.output_size:
+                raise ValueError(f"append_one_layer: {name} must be [{x.shape[0]}, heads, head_dim] of {self.output_size} elements a token")
+        d = self._decode(x, self._use_key(x)[0], layer_id, (0, 1, 2))
+        append_kv(q_out, q, k, v, k_cache, v_cache, positions, slots, cos, sin, *(y.view(t.shape) for y, t in zip(d, (q, k, v))),
+                  interleaved=interleaved, status=status)
 
     def _decode(self, x, where, layer_id, projs):
         """x ``[bsz, H]``; token ``t`` uses slot ``select_inds[bsz-1][t]`` (lora_gpu.py:137-138)."""

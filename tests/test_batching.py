@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from ae296_b200.batching import delta_cost_us, order_by_adapter, plan_for_requests
+from ae296_b200.batching import delta_cost_us, order_by_adapter, plan_for_requests, prefix_groups
 
 
 def test_order_is_stable_and_groups_adapters():
@@ -11,6 +11,21 @@ def test_order_is_stable_and_groups_adapters():
     o = order_by_adapter(ids)
     assert list(o) == [3, 1, 4, 0, 2, 5]
     assert list(np.asarray(ids)[o]) == [0, 2, 2, 5, 5, 5]
+
+
+@pytest.mark.parametrize("ids,starts,adapters", [([], [0], []), ([7], [0, 1], [7]), ([0, 2, 2, 5, 5, 5], [0, 1, 3, 6], [0, 2, 5]),
+                                                 ([3, 3, 3], [0, 3], [3]), ([-1, -1, 4, -1], [0, 2, 3, 4], [-1, 4, -1])])
+def test_prefix_groups_are_the_runs_of_one_adapter(ids, starts, adapters):
+    s, a = prefix_groups(ids)
+    assert s.dtype == np.int32 and list(s) == starts and list(a) == adapters
+
+
+def test_prefix_groups_of_an_ordered_batch_name_each_adapter_once():
+    ids = np.random.default_rng(0).integers(0, 40, 300)
+    s, a = prefix_groups(ids[order_by_adapter(ids)])
+    assert list(a) == sorted(set(ids.tolist())) and list(np.diff(s)) == [(ids == x).sum() for x in a]
+    with pytest.raises(ValueError, match="per request"):
+        prefix_groups([[1, 2]])
 
 
 def test_cost_grows_with_distinct_adapters_and_ranks_not_with_repeats():

@@ -398,6 +398,34 @@ def test_int4_inner_sizes_that_no_step_divides(K):
         check_int4(int4_case(K, T, K, 50, 32, "fp16"))
 
 
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("T", [8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 129])
+def test_int4_token_counts_around_the_tiles(T, group):
+    check_int4(int4_case(T, T, 512, 136, group, "bf16"))
+
+
+@pytest.mark.parametrize("T", [1, 12, 40])
+@pytest.mark.parametrize("K,group", [(1152, 32), (1152, 128), (1088, 64), (2048, 32), (512, 128)])
+def test_int4_factors_at_odd_addresses(T, K, group):
+    """Scales two bytes and zeros one byte behind a boundary, and rows of them that no word divides."""
+    s = int4_case(K + T, T, K, 140, group, "fp16")
+    for name in ("scales", "zeros"):
+        room = torch.full((s[name].numel() + 9,), 3, dtype=s[name].dtype, device="cuda")
+        s[name] = room[1:-8].view(s[name].shape).copy_(s[name])
+        assert s[name].data_ptr() % 4 != 0
+    check_int4(s)
+
+
+@pytest.mark.parametrize("T", [1, 9])
+def test_int4_scales_at_the_ends_of_their_type(T):
+    for dtype, sizes in (("fp16", (2.0 ** -24, 65504.0)), ("bf16", (2.0 ** -126, 2.0 ** 127))):
+        s = int4_case(11, T, 256, 64, 64, dtype, f32=True)
+        for size in sizes:
+            s["scales"].fill_(size)
+            s["x"].copy_(randn(torch.Generator().manual_seed(5), T, 256, dtype=TYPES[dtype], std=2.0 ** -4 if size < 1 else 2.0 ** -14))
+            check_int4(s)
+
+
 def test_int4_strided_rows_and_add_in_place():
     s = int4_case(3, 5, 512, 100, 64, "bf16", add=True)
     wide, out = torch.zeros(5, 600, dtype=torch.bfloat16, device="cuda"), torch.full((5, 131), 4.0, dtype=torch.bfloat16, device="cuda")
@@ -495,6 +523,50 @@ def test_a_layer_step_stage_by_stage():
         within(f64(got), w, half_step(a.dt) * np.abs(w) + 1e-5)
     check_attend(dict(a.cache, q=a.q, out=torch.empty_like(a.q)))
     check_int4(dict(a.o_w, x=a.cache["out"].flatten(1), y=a.y.clone(), add=a.x))
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_the_layer_object_appends_its_deltas(dtype):
+    """append_one_layer is the three deltas and the append, from whatever stream and in a captured graph."""
+    dt, H, T, D = TYPES[dtype], 512, 12, 64
+    torch.manual_seed(9)
+    obj = L.Lora_GPU({"n_layers": 2, "batch_size": 16, "lora_rank": 16, "hidden_dim": H, "tp_degree": 1, "max_prefill_batch_size": 2}, dtype=dt)
+    for pool in (obj.q_down, obj.q_up, obj.k_down, obj.k_up, obj.v_down, obj.v_up):
+        pool.copy_(torch.randn_like(pool) * 0.1)
+    s = append_case(61, T, H // D, H // D, D, D, 16, dtype, deltas=False)
+    for c in (s["k_cache"], s["v_cache"]):
+        c.zero_()
+    x = randn(torch.Generator().manual_seed(62), T, H, dtype=dt)
+    obj.set_indices(torch.randint(0, 16, (T,), device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+    d = [f(x, 1).view(T, -1, D).clone() for f in (obj.invoke_one_layer_q, obj.invoke_one_layer_k, obj.invoke_one_layer_v)]
+    assert all(t.abs().max() > 0 for t in d)
+    outs = ("q_out", "k_cache", "v_cache")
+    check_append(dict(s, dq=d[0], dk=d[1], dv=d[2]))
+    want = [s[n].clone() for n in outs]
+    rest = [s[n] for n in ("q_out", "q", "k", "v", "k_cache", "v_cache", "positions", "slots", "cos", "sin")]
+
+    def check():
+        torch.cuda.synchronize()
+        for n, w in zip(outs, want):
+            assert torch.equal(s[n], w)
+            s[n].zero_()
+
+    for n in outs:
+        s[n].zero_()
+    obj.append_one_layer(x, 1, *rest)
+    check()
+    with torch.cuda.stream(torch.cuda.Stream()):
+        obj.append_one_layer(x, 1, *rest)
+    check()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        obj.append_one_layer(x, 1, *rest)
+    graph.replay()
+    check()
+    with pytest.raises(ValueError, match="q must be"):
+        obj.append_one_layer(x, 1, s["q_out"], s["q"][:, :4], *rest[2:])
+    with pytest.raises(ValueError, match="k must be"):
+        obj.append_one_layer(x[:5], 1, s["q_out"], s["q"][:5], *rest[2:])
 
 
 def test_a_captured_step_follows_its_inputs_and_eager_calls_between_replays():
