@@ -37,18 +37,6 @@ __device__ __forceinline__ void ldsm4t(unsigned addr, unsigned (&r)[4]) {
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
-// Entity e of this kernel: group e, or request e - n_groups
-__device__ __forceinline__ Entity entity_of(const AttnParams& p, int e, bool usable, int& bad) {
-    if (e < p.a.n_groups) return group_of<kAttnRows, kKeys, false>(p, e, usable, bad);
-    Entity t;
-    t.first = e - p.a.n_groups;
-    t.rows = p.per;
-    t.tiles = p.req_tiles;
-    t.keys = clamped_keys(p, p.a.lens[t.first], p.a.max_pages, bad);
-    t.chunks = (t.keys + kKeys - 1) / kKeys;
-    return t;
-}
-
 template <int D>
 __device__ __forceinline__ unsigned chunk_addr(unsigned base, int row, int chunk) {
     return base + row * (D * 2) + ((chunk ^ (row & 7)) << 4);
@@ -74,22 +62,31 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
     __shared__ unsigned long long warp_sum[kWarps];
     __shared__ int key_mask[kWarps][R::kStages];
     __shared__ int bad_all;
+    __shared__ unsigned long long wide_sum;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // Behind the wide kernel, which leaves alone what this one reads, only its end is waited for (at this one's own):
-    // whatever came before the wide kernel is complete when a block of this one runs.
+    // Beside the wide kernel, which leaves alone what this one reads, only its end is waited for (at this one's own): whatever came
+    // before the wide kernel is complete when a block of this one runs.  Blocks that find no SM free run behind it, and end at once.
     if (!p.wide_tiles) {
         pdl_wait_prior();
         if (tid == 0) pdl_launch_dependents();
     }
-    if (tid == 0) bad_all = 0;
+    if (tid == 0) { bad_all = 0; wide_sum = 0; }
     __syncthreads();
+    int ignored = 0;
+    if (p.wide_tiles)
+        add_units<kThreads>(p.a.n_groups, &wide_sum, [&](int e) {
+            const Entity t = group_of<kWideRows, kWideKeys, true>(p, e, true, ignored);
+            return (unsigned long long)(t.tiles * t.chunks);
+        });
     // units before each entity, row tiles before each group; written out once for the join
     const int n_ent = p.a.n_groups + p.a.n_requests;
     const bool groups = scan_units<kThreads>(n_ent, p.a.n_groups, su, st, warp_sum, &bad_all, [&](int e, bool usable, int& bad) {
-        const Entity t = entity_of(p, e, usable, bad);
+        const Entity t = split_entity(p, e, usable, bad);
         return ((unsigned long long)(e < p.a.n_groups ? t.tiles : 0) << 32) | (unsigned)(t.tiles * t.chunks);
     });
+    const int n_sm = gridDim.x, wide_sm = wide_share(groups ? (long long)wide_sum : 0, su[n_ent], n_sm), mine = max(1, n_sm - wide_sm);
     if (blockIdx.x == 0) {
+        if (tid == 0) { p.shares[0] = mine * kWarps; p.shares[1] = wide_sm; }
         for (int i = tid; i <= n_ent; i += kThreads) p.units[i] = su[i];
         for (int i = tid; i <= p.a.n_groups; i += kThreads) p.tiles[i] = groups ? st[i] : -1;
         if (tid == 0 && bad_all && p.a.status) atomicOr(p.a.status, bad_all);
@@ -97,9 +94,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
 
     const int n_kv = p.c.n_kv_heads;
     const long long total = (long long)su[n_ent] * n_kv;
-    const int workers = (int)min((long long)p.workers, total);
-    const int worker = warp * gridDim.x + blockIdx.x;        // neighbours in the work on different SMs
-    if (worker >= workers) {
+    const int workers = (int)min((long long)mine * kWarps, total);
+    const int worker = warp * mine + blockIdx.x;             // neighbours in the work on different SMs
+    if ((int)blockIdx.x >= mine || worker >= workers) {
         pdl_wait_prior();
         pdl_launch_dependents();
         return;
@@ -108,13 +105,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
     const long long u_end = unit_of_worker(total, worker + 1, workers);
     const unsigned ring = smem_u32(smem) + warp * R::kStages * R::kStage;
     const int g4 = lane >> 2, t4 = lane & 3;
-    int ignored = 0;
 
     while (u < u_end) {
         // ---- the item of unit u
         const int uh = (int)(u / n_kv);
         const int e = entity_at(su, n_ent, uh);
-        const Entity t = entity_of(p, e, groups, ignored);
+        const Entity t = split_entity(p, e, groups, ignored);
         long long r = u - (long long)n_kv * su[e];
         const int per_head = t.tiles * t.chunks;
         const int h = (int)(r / per_head);
@@ -281,7 +277,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     const int h = hq / p.per, i = hq - h * p.per, n_kv = p.c.n_kv_heads, n_g = p.a.n_groups;
     const int n_ent = n_g + p.a.n_requests;
     const long long total = (long long)p.units[n_ent] * n_kv;
-    const int workers = (int)min((long long)p.workers, total);
+    const int workers = (int)min((long long)p.shares[0], total);
 
     constexpr int V = D / 32;
     // The row's parts: those of its group's item (a wide tile of one stream's rows has a second part for each), then of its own.  Part
@@ -304,7 +300,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
                 const long long u0 = (long long)n_kv * units[lo] + (long long)h * all + (long long)tile * chunks;
                 const size_t item = (size_t)n_kv * before[lo] + (size_t)h * tiles + tile;
                 const long long sum = wide ? (long long)p.wide_units[n_g] * n_kv : total;
-                const int w = wide ? (int)min((long long)p.wide_workers, sum) : workers;
+                const int w = wide ? (int)min((long long)p.shares[1], sum) : workers;
                 const int w0 = worker_of_unit(sum, u0, w), n = worker_of_unit(sum, u0 + chunks - 1, w) - w0 + 1;
                 if (!wide) run[0] = {(item + w0) * kAttnRows + (r - tile * kAttnRows), kAttnRows, n};
                 else {
@@ -387,8 +383,7 @@ template <typename T, int D>
 cudaError_t launch_typed(const AttnParams& p0, int n_sm, cudaStream_t s) {
     AttnParams p = p0;
     const int grid = n_sm < kAttnMaxWorkers / kWarps ? n_sm : kAttnMaxWorkers / kWarps;
-    p.workers = grid * kWarps;
-    p.wide_workers = n_sm < kWideMaxWorkers ? n_sm : kWideMaxWorkers;
+    p.grid = grid;
     const size_t smem = Ring<D>::kBytes + 4 * ((size_t)2 * p.a.n_groups + p.a.n_requests + 2);
     cudaError_t e = cudaSuccess;
     if (p.wide_tiles) {

@@ -47,6 +47,7 @@ struct WideShared {
     unsigned long long full[kMaxRing], empty[kMaxRing], q_ready[2], s_full[2], p_ready[2], o_full[2];
     unsigned long long warp_sum[kThreads / 32];
     unsigned tmem, err;
+    unsigned long long split_sum[2];             // of the groups, of the requests
     int bad, pad;
 };
 static_assert(sizeof(WideShared) % 16 == 0, "the scan's arrays follow");
@@ -112,8 +113,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (tid == 0) { sh.err = 0u; sh.bad = 0; }
+    if (tid < 2) sh.split_sum[tid] = 0;
     __syncthreads();
     const int n_g = p.a.n_groups, n_kv = p.c.n_kv_heads;
+    for (int k = 0; k < 2; ++k)
+        add_units<kThreads>(k == 0 ? n_g : p.a.n_requests, &sh.split_sum[k], [&](int e) {
+            int ignored = 0;
+            const Entity t = split_entity(p, k == 0 ? e : n_g + e, true, ignored);
+            return (unsigned long long)(t.tiles * t.chunks);
+        });
     const bool usable = scan_units<kThreads>(n_g, n_g, su, st, sh.warp_sum, &sh.bad, [&](int e, bool ok, int& bad) {
         const Entity t = group_of<kWideRows, kWideKeys, true>(p, e, ok, bad);
         return ((unsigned long long)t.tiles << 32) | (unsigned)(t.tiles * t.chunks);
@@ -121,7 +129,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     if (blockIdx.x == 0)
         for (int i = tid; i <= n_g; i += kThreads) { p.wide_units[i] = su[i]; p.wide_tile[i] = st[i]; }
     const long long total = (long long)su[n_g] * n_kv;
-    const int workers = (int)min((long long)p.wide_workers, total);
+    const int share = wide_share(su[n_g], (long long)((usable ? sh.split_sum[0] : 0) + sh.split_sum[1]), gridDim.x);
+    const int workers = (int)min((long long)share, total);
     if ((int)blockIdx.x >= workers) return;
     const long long u_first = unit_of_worker(total, blockIdx.x, workers), u_end = unit_of_worker(total, blockIdx.x + 1, workers);
     auto part_at = [&](long long u) { return part_of(p, su, st, usable, u, u_end); };
@@ -474,7 +483,21 @@ cudaError_t launch_ring(const AttnParams& p, size_t scan, cudaStream_t s) {
     const size_t smem = Wide<D, RING>::kBytes + sizeof(WideShared) + scan + 1024;
     const cudaError_t e = allow_smem<attn_wide_kernel<T, D, RING>>((int)smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(attn_wide_kernel<T, D, RING>, p.wide_workers, kThreads, smem, s, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)p.grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    // Neighbours in pairs, so that two SMs that share their way to memory do the same: else the split kernel's reading slows some of
+    // these blocks down and all wait for those (256 requests of one prefix of 16384 tokens: 371 us instead of 318 us).
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.grid % 2 == 0 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, attn_wide_kernel<T, D, RING>, p);
 }
 template <typename T>
 cudaError_t launch_typed(const AttnParams& p, cudaStream_t s) {

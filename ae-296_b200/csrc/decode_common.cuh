@@ -32,13 +32,13 @@ struct AttnParams {
     int req_tiles;         // row tiles of a request
     int req_rows;          // rows of a request's partial result
     int max_group_tiles;   // of all groups together
-    int workers;
+    int grid;              // SMs
     int wide_tiles;        // at most, of all groups together; 0: no group can be that large
-    int wide_workers;
     float scale_log2;
     int* units;            // [n_groups + n_requests + 1] units of a cache head before each entity
     int* tiles;            // [n_groups + 1] row tiles before each group
     int *wide_units, *wide_tile;   // the same of the wide kernel, [n_groups + 1] both
+    int* shares;           // [2] of the split kernel's warps and of the wide kernel's blocks that work
     float* part;           // partial results: rows of head_dim sums, then of (maximum, sum)
     float2* part_ml;
 };
