@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
     const int f_row = tid >> 1, f_first = (tid & 1) * kHalf;
     const long long f_at = (long long)min(row0 + f_row, a.n_out - 1) * n_groups;
     static_assert(kHalf == 4, "two words of scales and one of zeros");
-    const bool words = n_groups % 4 == 0 && (reinterpret_cast<uintptr_t>(a.scales) & 7) == 0 && (reinterpret_cast<uintptr_t>(a.zeros) & 3) == 0;
+    // (a part may begin in the middle of four groups)
+    const bool words = n_groups % 4 == 0 && s0 * (kStageK / G) % 4 == 0 && (reinterpret_cast<uintptr_t>(a.scales) & 7) == 0 && (reinterpret_cast<uintptr_t>(a.zeros) & 3) == 0;
     const unsigned short* scales = static_cast<const unsigned short*>(a.scales) + f_at;
     const unsigned char* zeros = static_cast<const unsigned char*>(a.zeros) + f_at;
     uint2 sc;

@@ -399,12 +399,17 @@ def test_int4_inner_sizes_that_no_step_divides(K):
 
 
 @pytest.mark.parametrize("group", [32, 64, 128])
-@pytest.mark.parametrize("T", [8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 129])
+@pytest.mark.parametrize("T", [1, 2, 3, 4, 5, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 129])
 def test_int4_token_counts_around_the_tiles(T, group):
     check_int4(int4_case(T, T, 512, 136, group, "bf16"))
 
 
-@pytest.mark.parametrize("T", [1, 12, 40])
+@pytest.mark.parametrize("T,K,N", [(1, 49152, 9), (1, 49184, 9), (2, 24576, 33), (2, 25600, 33), (4, 12288, 130), (3, 13312, 130), (1, 1024, 9001), (3, 2080, 5000)])
+def test_int4_few_tokens_of_long_rows_and_of_many(T, K, N):
+    check_int4(int4_case(K + N, T, K, N, 32, "bf16", add=True))
+
+
+@pytest.mark.parametrize("T", [1, 3, 12, 40])
 @pytest.mark.parametrize("K,group", [(1152, 32), (1152, 128), (1088, 64), (2048, 32), (512, 128)])
 def test_int4_factors_at_odd_addresses(T, K, group):
     """Scales two bytes and zeros one byte behind a boundary, and rows of them that no word divides."""
@@ -424,6 +429,12 @@ def test_int4_scales_at_the_ends_of_their_type(T):
             s["scales"].fill_(size)
             s["x"].copy_(randn(torch.Generator().manual_seed(5), T, 256, dtype=TYPES[dtype], std=2.0 ** -4 if size < 1 else 2.0 ** -14))
             check_int4(s)
+
+
+@pytest.mark.parametrize("T", [1, 5, 8, 9, 33])
+@pytest.mark.parametrize("K,group", [(5120, 128), (5120, 64), (6656, 128), (6656, 32)])
+def test_int4_parts_that_begin_inside_a_word_of_factors(T, K, group):
+    check_int4(int4_case(K + T, T, K, 40, group, "bf16"))
 
 
 def test_int4_strided_rows_and_add_in_place():
