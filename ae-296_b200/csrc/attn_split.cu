@@ -425,7 +425,7 @@ cudaError_t launch_typed(const AttnParams& p0, int n_sm, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     e = launch_pdl(attn_split_kernel<T, D>, grid, kThreads, smem, s, p);
     if (e != cudaSuccess) return e;
-    // Eight warps for a row where the rows are few: there its parts are many (32 rows of 4096 keys: 11.7 us with one warp, 10.1 us; 4096
+    // Eight warps for a row where the rows are few: there its parts are many (32 rows of 311 keys: 11.7 us with one warp, 10.1 us; 4096
     // rows of 8704 keys: 69 us with one, 89 us with eight).
     const unsigned rows = (unsigned)p.a.n_requests * p.a.n_heads;
     if (rows <= (unsigned)n_sm * 2) return launch_pdl(attn_join_kernel<T, D, kJoinWarps>, rows, kJoinWarps * 32, 0, s, p);

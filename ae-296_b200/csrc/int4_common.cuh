@@ -1,4 +1,4 @@
-// What the two kernels of the products with 4-bit weights share (sm_100a).
+// What the kernels of the products with 4-bit weights share (sm_100a).
 #pragma once
 
 #include <initializer_list>
@@ -170,6 +170,8 @@ inline bool encode_int4(Int4Params& p, uint32_t tokens, uint32_t panels) {
                        : encode_map(&p.x, a.x, {k, t}, {(uint64_t)a.x_row}, {64, tokens}));
 }
 
+bool int4_rows_take(const b200_int4& a);      // one or two tokens, as long as x fits and the product is not too large
+cudaError_t launch_int4_rows(const b200_int4& a, int dtype, int y_f32, int n_sm, cudaStream_t s);
 cudaError_t launch_int4_few(const b200_int4& a, int dtype, int y_f32, int n_sm, cudaStream_t s);      // up to kInt4Few tokens
 constexpr int kInt4Few = 8;
 

@@ -1,4 +1,4 @@
-// Products of at most eight tokens with 4-bit weights (see int4_linear.cu for the mathematics): mma.sync, 16 weight rows by eight
+// Products of three to eight tokens with 4-bit weights (see int4_linear.cu for the mathematics): mma.sync, 16 weight rows by eight
 // tokens.  For so few tokens the tensor core of tcgen05 takes longer over a tile (45 cycles for 2048 weights, whatever the
 // tokens) than the codes take to arrive; a warp's own multiplication takes 256 weights every three cycles and has its numbers
 // in registers.

@@ -301,6 +301,7 @@ cudaError_t launch_typed(const b200_int4& a, int y_f32, int n_sm, cudaStream_t s
 }  // namespace
 
 cudaError_t launch_int4(const b200_int4& a, int dtype, int y_f32, int n_sm, cudaStream_t s) {
+    if (int4_rows_take(a)) return launch_int4_rows(a, dtype, y_f32, n_sm, s);
     if (a.n_tokens <= kInt4Few) return launch_int4_few(a, dtype, y_f32, n_sm, s);
     return dtype == B200_LORA_F16 ? launch_typed<__half>(a, y_f32, n_sm, s) : launch_typed<__nv_bfloat16>(a, y_f32, n_sm, s);
 }
