@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kThreads, kBlocks) int4_rows_kernel(const __gr
     const int row_groups = (a.n_out - 1) / kRows + 1, n_groups = a.n_in / a.group, workers = gridDim.x * per_block;
     int rg = blockIdx.x * per_block + warp / parts;           // group of kRows rows
     const int s0 = p.steps * part / parts, n_steps = p.steps * (part + 1) / parts - s0;
-    auto row_of = [&](int rg, int r) { return min((long long)rg * kRows + r, a.n_out - 1ll); };
+    auto row_of = [&](int rg, int r) { return (long long)(rg * kRows + min(r, a.n_out - 1 - rg * kRows)); };
     auto codes_of = [&](int rg, int r, int col) { return static_cast<const unsigned char*>(a.codes) + row_of(rg, r) * (a.n_in / 2) + col / 2; };
     {
         // the first codes are on their way to L2 while the predecessor ends (what it may still write, L2 sees too)
@@ -151,9 +151,8 @@ __global__ void __launch_bounds__(kThreads, kBlocks) int4_rows_kernel(const __gr
                 if (lane == r * TOKENS + t) sums[warp][lane] = acc[r][t];
             }
         if (parts > 1) __syncthreads(); else __syncwarp();
-        const int r = lane / TOKENS, t = lane % TOKENS;
-        const long long row = (long long)rg * kRows + r;
-        if (part == 0 && r < kRows && rg < row_groups && row < a.n_out) {
+        const int r = lane / TOKENS, t = lane % TOKENS, row0 = rg < row_groups ? rg * kRows : 0, row = row0 + r;
+        if (part == 0 && r < kRows && rg < row_groups && r < a.n_out - row0) {
             float f = 0.f;
             for (int w = 0; w < parts; ++w) f += sums[warp + w][lane];
             const long long to = (long long)t * a.y_row + row, from = (long long)t * a.add_row + row;
