@@ -421,7 +421,7 @@ cudaError_t launch_typed(const AttnParams& p0, int n_sm, cudaStream_t s) {
         e = launch_attention_wide(p, std::is_same_v<T, __half> ? B200_LORA_F16 : B200_LORA_BF16, s);
         if (e != cudaSuccess) return e;
     }
-    e = allow_smem<attn_split_kernel<T, D>>((int)smem);
+    e = allow_smem<attn_split_kernel<T, D>>();
     if (e != cudaSuccess) return e;
     e = launch_pdl(attn_split_kernel<T, D>, grid, kThreads, smem, s, p);
     if (e != cudaSuccess) return e;

@@ -52,7 +52,6 @@ struct WideShared {
 };
 static_assert(sizeof(WideShared) % 16 == 0, "the scan's arrays follow");
 constexpr int kNoPage = -0x7fffffff - 1;         // of a key behind the prefix
-constexpr int kSmemLimit = 232448;                // of a block
 
 // one of the barrier's arrivals, once this thread's copies so far have landed
 __device__ __forceinline__ void arrive_when_copied(unsigned b) {
@@ -481,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
 template <typename T, int D, int RING>
 cudaError_t launch_ring(const AttnParams& p, size_t scan, cudaStream_t s) {
     const size_t smem = Wide<D, RING>::kBytes + sizeof(WideShared) + scan + 1024;
-    const cudaError_t e = allow_smem<attn_wide_kernel<T, D, RING>>((int)smem);
+    const cudaError_t e = allow_smem<attn_wide_kernel<T, D, RING>>();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.grid);

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "b200_decode.h"
+#include "entry_common.cuh"
 #include "lora_common.cuh"
 
 namespace b200lora {

@@ -142,7 +142,7 @@ inline int int4_split(long long tiles, int stages, int at_once) {
 // launch of a cluster of p.split blocks along y
 template <auto KERNEL>
 inline cudaError_t launch_int4_kernel(const Int4Params& p, dim3 grid, int threads, size_t smem, cudaStream_t s) {
-    const cudaError_t e = allow_smem<KERNEL>((int)smem);
+    const cudaError_t e = allow_smem<KERNEL>();
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;

@@ -175,7 +175,7 @@ cudaError_t launch_tokens(const b200_int4& a, int y_f32, int n_sm, cudaStream_t 
     while (p.parts < kWarps && 2 * p.parts <= p.steps && (row_groups * 2 * p.parts + kWarps - 1) / kWarps <= slots) p.parts *= 2;
     const long long blocks = (row_groups * p.parts + kWarps - 1) / kWarps;
     const size_t smem = (size_t)TOKENS * p.steps * kStep * 2;
-    const cudaError_t e = allow_smem<int4_rows_kernel<T, TOKENS>>((int)smem);
+    const cudaError_t e = allow_smem<int4_rows_kernel<T, TOKENS>>();
     if (e != cudaSuccess) return e;
     return launch_pdl(int4_rows_kernel<T, TOKENS>, dim3((unsigned)(blocks < slots ? blocks : slots)), dim3(kThreads), smem, s, p);
 }

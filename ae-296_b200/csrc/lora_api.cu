@@ -4,6 +4,7 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "entry_common.cuh"
 #include "lora_common.cuh"
 
 using namespace b200lora;

@@ -7,8 +7,6 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <atomic>
-#include <initializer_list>
 #include <utility>
 
 #include "b200_lora.h"
@@ -302,24 +300,6 @@ inline cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, dim3 block, s
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-
-// ---- shared by the entry points (lora_api.cu) ------------------------------------------------
-int cuda_fail(cudaError_t e);             // keeps the error's text for b200_lora_last_cuda_error; returns B200_LORA_ERR_CUDA
-int sm_count();                           // of the current device
-bool encode_map(CUtensorMap* out, const void* base, std::initializer_list<uint64_t> extents, std::initializer_list<uint64_t> strides,
-                std::initializer_list<uint32_t> box);
-
-// Dynamic shared memory beyond 48 KB has to be allowed once per kernel and device; KERNEL distinguishes the flags.
-template <auto KERNEL>
-inline cudaError_t allow_smem(int bytes) {
-    static std::atomic<int> allowed[64];
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess || (dev >= 0 && dev < 64 && allowed[dev].load(std::memory_order_relaxed) >= bytes)) return e;
-    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev >= 0 && dev < 64) allowed[dev].store(bytes, std::memory_order_relaxed);
-    return e;
 }
 
 // ---- launchers implemented by the kernel files ---------------------------------------------
