@@ -8,6 +8,13 @@ namespace b200lora {
 
 namespace {
 
+// a / b of numbers that are not negative and seldom have more than 32 bits: a division of 64-bit ones takes some 400 cycles
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((unsigned)a / (unsigned)b) : a / b;
+}
+// Request of a group's row: row / per by multiplication, exact as long as row * per < 2^32 (rows <= 4096 * per, per <= 1024)
+__device__ __forceinline__ int request_of_row(const AttnParams& p, int row) { return p.per == 1 ? row : (int)__umulhi((unsigned)row, p.per_inverse); }
+
 struct Entity { int rows, tiles, chunks, keys, first; };     // first: request of the first row
 
 __device__ __forceinline__ int clamped_keys(const AttnParams& p, int n, int pages, int& bad) {
@@ -16,7 +23,7 @@ __device__ __forceinline__ int clamped_keys(const AttnParams& p, int n, int page
     return n < 0 ? 0 : n > most ? most : n;
 }
 // Group e, cut into tiles of TILE rows and chunks of KEYS keys.  `usable` false: the group starts cannot be used and no
-// group has rows.  Groups of more than kAttnRows rows are the wide kernel's, the others the split kernel's.
+// group has rows.  Groups of more than kWideFrom rows are the wide kernel's, the others the split kernel's.
 template <int TILE, int KEYS, bool WIDE>
 __device__ __forceinline__ Entity group_of(const AttnParams& p, int e, bool usable, int& bad) {
     Entity t;
@@ -25,7 +32,7 @@ __device__ __forceinline__ Entity group_of(const AttnParams& p, int e, bool usab
     if (!fine) bad |= B200_DECODE_BAD_GROUPS;
     t.first = s0;
     t.rows = fine && usable ? (s1 - s0) * p.per : 0;
-    if ((t.rows > kAttnRows) != WIDE) t.rows = 0;
+    if ((t.rows > kWideFrom) != WIDE) t.rows = 0;
     t.tiles = (t.rows + TILE - 1) / TILE;
     t.keys = clamped_keys(p, p.a.prefix_lens[e], p.a.max_prefix_pages, bad);
     if (t.rows == 0) t.keys = 0;
@@ -64,7 +71,7 @@ constexpr int kWideCost = 18;
 __device__ __forceinline__ int wide_share(long long wide, long long split, int n) {
     if (wide == 0 || split == 0) return wide == 0 ? 0 : n;
     const long long w = wide * kWideCost;
-    const int x = 2 * (int)((w * n + (w + split)) / (2 * (w + split))), least = n / 32 * 2;
+    const int x = 2 * (int)quotient(w * n + (w + split), 2 * (w + split)), least = n / 32 * 2;
     return max(1, min(max(x, least), n - least));
 }
 
@@ -117,9 +124,9 @@ __device__ __forceinline__ int entity_at(const int* su, int n, int uh) {
     return lo;
 }
 
-__device__ __forceinline__ long long unit_of_worker(long long total, int w, int workers) { return total * w / workers; }
+__device__ __forceinline__ long long unit_of_worker(long long total, int w, int workers) { return quotient(total * w, workers); }
 __device__ __forceinline__ int worker_of_unit(long long total, long long u, int workers) {
-    return (int)(((u + 1) * workers - 1) / total);
+    return (int)quotient((u + 1) * workers - 1, total);
 }
 
 __device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool valid) {

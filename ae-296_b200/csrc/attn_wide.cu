@@ -19,6 +19,13 @@
 // Warps 0..3 and 4..7: the streams.  Warp 8: one thread issues the multiplications.  Warps 9..11 bring keys and values
 // into a ring of blocks by asynchronous 16-byte copies in the 128-byte swizzled layout the multiplications read, page
 // by page, whatever the page size, with zeros in place of keys behind the prefix or in pages that do not exist.
+//
+// 256 requests of 64 heads over 8 of 128, a prefix of 16384 tokens: a unit of 256 rows takes an SM some 4500 cycles, of which the
+// multiplications need 2048 and the exponentials of a stream's warps 1500, while each waits for the other's result twice: 0.83
+// PFLOP/s over the whole GPU, half of what a library product reaches.  64 requests, a prefix of 8192: 55 us of which 12 are start and
+// end (queries, TMEM, the partial rows).  Tried and taken back: two threads a row (half the row each, no registers for more
+// in flight: 328 us against 314 us in all), scores kept in registers (spills: 587 us against 325 us).
+//
 // Every wait is bounded: on expiry control flow stays as it is, and the outputs become NaN.
 #include <type_traits>
 
@@ -69,12 +76,12 @@ __device__ __forceinline__ Part part_of(const AttnParams& p, const int* su, cons
     Part t;
     int ignored = 0;
     const int n_kv = p.c.n_kv_heads;
-    const int uh = (int)(u / n_kv);
+    const int uh = (int)quotient(u, n_kv);
     t.g = entity_at(su, p.a.n_groups, uh);
     const Entity e = group_of<kWideRows, kWideKeys, true>(p, t.g, usable, ignored);
     const int per_head = e.tiles * e.chunks;
     const long long of_entity = u - (long long)n_kv * su[t.g];
-    t.h = (int)(of_entity / per_head);
+    t.h = (int)quotient(of_entity, per_head);
     const int rest = (int)(of_entity - (long long)t.h * per_head);
     t.tile = rest / e.chunks;
     t.b0 = rest - t.tile * e.chunks;
@@ -111,6 +118,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));
     if (tid == 0) { sh.err = 0u; sh.bad = 0; }
     if (tid < 2) sh.split_sum[tid] = 0;
     __syncthreads();
@@ -130,15 +138,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     const long long total = (long long)su[n_g] * n_kv;
     const int share = wide_share(su[n_g], (long long)((usable ? sh.split_sum[0] : 0) + sh.split_sum[1]), gridDim.x);
     const int workers = (int)min((long long)share, total);
-    if ((int)blockIdx.x >= workers) return;
-    const long long u_first = unit_of_worker(total, blockIdx.x, workers), u_end = unit_of_worker(total, blockIdx.x + 1, workers);
-    auto part_at = [&](long long u) { return part_of(p, su, st, usable, u, u_end); };
-
-    if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&sh.tmem);
+    if ((int)blockIdx.x >= workers) {
+        if (warp == 8) tmem_dealloc(tmem);
+        return;
+    }
+    const long long u_first = unit_of_worker(total, blockIdx.x, workers), u_end = unit_of_worker(total, blockIdx.x + 1, workers);
+    auto part_at = [&](long long u) { return part_of(p, su, st, usable, u, u_end); };
+
     const unsigned ring = smem_u32(smem) + 2 * W::kQ;
     // The ring's order within a part: where the streams share blocks, K0 V0 K1 V1 ...; where they take them in turns,
     // K0 K1 V0 K2 V1 K3 ...: what the multiplications need next always comes next.
@@ -318,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             // ---- queries to shared memory (the stream's last multiplication that reads them is complete)
             if (b_first < t.n) {
                 const unsigned qa = smem_u32(smem) + s * W::kQ;
-                constexpr int kPieces = D / 8, kBatch = 8;
+                constexpr int kPieces = D / 8, kBatch = kPieces;
                 const int c = row % kPieces;
 #pragma unroll
                 for (int i0 = 0; i0 < kPieces; i0 += kBatch) {
@@ -328,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                         const int r = ((i0 + i) * kStreamRows + row) / kPieces, in_tile = t.dual ? s * kStreamRows + r : r;
                         v[i] = make_uint4(flip, flip, flip, flip);
                         if (in_tile < t.rows) {
-                            const int ra = t.tile * kWideRows + in_tile, request = ra / p.per;
+                            const int ra = t.tile * kWideRows + in_tile, request = request_of_row(p, ra);
                             v[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.a.q) + (long long)(t.first + request) * p.a.q_row +
                                                                     (long long)(t.h * p.per + ra - request * p.per) * p.a.q_head + c * 8);
                         }

@@ -24,13 +24,14 @@ int attention_sizes(AttnParams& p) {
         (p.c.head_dim != 64 && p.c.head_dim != 128))
         return B200_LORA_ERR_DIM;
     p.per = p.a.n_heads / p.c.n_kv_heads;
+    p.per_inverse = (unsigned)(((1ull << 32) + p.per - 1) / p.per);
     p.req_tiles = (p.per + kAttnRows - 1) / kAttnRows;
     p.req_rows = p.per < kAttnRows ? p.per : kAttnRows;
     const int rows = p.a.n_requests * p.per;                  // at most 4096 * 1024
-    const bool wide = p.a.n_groups > 0 && rows > kAttnRows;
-    // groups of at most kAttnRows rows, and wide ones (of which there are fewer than rows / kAttnRows)
-    p.max_group_tiles = p.a.n_groups;
-    const int wide_groups = rows / (kAttnRows + 1);
+    const bool wide = p.a.n_groups > 0 && rows > kWideFrom;
+    // groups of at most kWideFrom rows, and wide ones (of which there are fewer than rows / kWideFrom)
+    p.max_group_tiles = p.a.n_groups + (kWideFrom > kAttnRows && p.a.n_groups > 0 ? rows / kAttnRows : 0);
+    const int wide_groups = rows / (kWideFrom + 1);
     p.wide_tiles = wide ? (rows + kWideRows - 1) / kWideRows + (p.a.n_groups < wide_groups ? p.a.n_groups : wide_groups) : 0;
     return B200_LORA_OK;
 }

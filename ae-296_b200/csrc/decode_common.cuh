@@ -19,8 +19,11 @@ cudaError_t launch_kv_append(const b200_append& a, const b200_kv_cache& c, int d
 constexpr int kAttnKeys = 16;
 constexpr int kAttnRows = 16;
 constexpr int kAttnMaxWorkers = 2048;
-// Groups of more than kAttnRows rows go to the wide kernel: units of kWideKeys keys for tiles of kWideRows rows, one
-// worker per SM.
+// Groups of more than kWideFrom rows go to the wide kernel: units of kWideKeys keys for tiles of kWideRows rows, one
+// worker per SM.  With 64 heads over 8 of 128, 32 groups of 4 requests (32 rows) over prefixes of 2048 tokens take 103 us in the split kernel
+// (two tiles, of which the second finds the keys in L2) and 121 us in the wide one, 32 groups of 8 (64 rows) 190 and 141 us; one group
+// over 16384 tokens 32 and 35 us (32 rows), 55 and 43 us (64 rows).
+constexpr int kWideFrom = 32;
 constexpr int kWideKeys = 128;
 constexpr int kWideRows = 256;
 constexpr int kWideMaxWorkers = 256;
@@ -29,6 +32,7 @@ struct AttnParams {
     b200_attention a;
     b200_kv_cache c;
     int per;               // query heads of a cache head
+    unsigned per_inverse;  // 2^32 / per, rounded up
     int page_shift;
     int req_tiles;         // row tiles of a request
     int req_rows;          // rows of a request's partial result

@@ -173,6 +173,8 @@ inline bool encode_int4(Int4Params& p, uint32_t tokens, uint32_t panels) {
 bool int4_rows_take(const b200_int4& a);      // one or two tokens, as long as x fits and the product is not too large
 cudaError_t launch_int4_rows(const b200_int4& a, int dtype, int y_f32, int n_sm, cudaStream_t s);
 cudaError_t launch_int4_few(const b200_int4& a, int dtype, int y_f32, int n_sm, cudaStream_t s);      // up to kInt4Few tokens
+// Eight tokens there and nine on the tensor core's 128 rows by 16 tokens (int4_linear.cu): 4096 rows of 4096 columns, groups of 128, 8.8
+// and 8.0 us, 8192 of 8192 17.5 and 17.1 us; 1024 of 8192, groups of 32, 7.7 and 9.3 us, 32000 of 8192, groups of 64, 42 and 49 us.
 constexpr int kInt4Few = 8;
 
 }  // namespace b200lora

