@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     unsigned* err = &sh.err;
 
     pdl_wait_prior();
-    if (tid == 0) pdl_launch_dependents();
+    if (tid == 0) pdl_launch_dependents();       // (before TMEM: the split kernel, which follows, takes none)
     if (tid < kMaxRing) {
         if (tid < RING) { mbar_init(bar(sh.full[tid]), kCopyThreads + kCopyWarps); mbar_init(bar(sh.empty[tid]), 1); }
         if (tid < 2) {

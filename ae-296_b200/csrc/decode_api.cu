@@ -30,7 +30,7 @@ int attention_sizes(AttnParams& p) {
     const int rows = p.a.n_requests * p.per;                  // at most 4096 * 1024
     const bool wide = p.a.n_groups > 0 && rows > kWideFrom;
     // groups of at most kWideFrom rows, and wide ones (of which there are fewer than rows / kWideFrom)
-    p.max_group_tiles = p.a.n_groups + (kWideFrom > kAttnRows && p.a.n_groups > 0 ? rows / kAttnRows : 0);
+    p.max_group_tiles = p.a.n_groups * (kWideFrom / kAttnRows);
     const int wide_groups = rows / (kWideFrom + 1);
     p.wide_tiles = wide ? (rows + kWideRows - 1) / kWideRows + (p.a.n_groups < wide_groups ? p.a.n_groups : wide_groups) : 0;
     return B200_LORA_OK;
@@ -120,7 +120,7 @@ extern "C" int b200_int4_linear(const b200_int4* a, int32_t dtype, int32_t y_dty
     if (a->n_tokens == 0) return B200_LORA_OK;
     b200_int4 q = *a;
     if (a->n_tokens == 1) q.x_row = (a->n_in + 7) / 8 * 8;       // whatever it was said to be
-    if (q.x_row < a->n_in || a->n_tokens > 65535 * 64) return B200_LORA_ERR_DIM;
+    if (q.x_row < a->n_in || a->n_tokens > 65535 * 32) return B200_LORA_ERR_DIM;      // blocks along z
     const cudaError_t e = launch_int4(q, dtype, y_dtype == B200_LORA_F32, sm_count(), static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? B200_LORA_OK : cuda_fail(e);
 }

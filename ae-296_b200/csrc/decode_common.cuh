@@ -23,7 +23,7 @@ constexpr int kAttnMaxWorkers = 2048;
 // worker per SM.  With 64 heads over 8 of 128, 32 groups of 4 requests (32 rows) over prefixes of 2048 tokens take 103 us in the split kernel
 // (two tiles, of which the second finds the keys in L2) and 121 us in the wide one, 32 groups of 8 (64 rows) 190 and 141 us; one group
 // over 16384 tokens 32 and 35 us (32 rows), 55 and 43 us (64 rows).
-constexpr int kWideFrom = 32;
+constexpr int kWideFrom = 32;                     // a multiple of kAttnRows
 constexpr int kWideKeys = 128;
 constexpr int kWideRows = 256;
 constexpr int kWideMaxWorkers = 256;

@@ -93,6 +93,8 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.err = 0u;
     }
+    // TMEM only after the wait: a predecessor may let this block come before it has its own, and would then wait for this one's
+    pdl_wait_prior();
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)), "n"(S::kAlloc) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -101,7 +103,6 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
     __syncthreads();
     tc_fence_after();
     const unsigned tmem = *reinterpret_cast<volatile unsigned*>(&sh.tmem);
-    pdl_wait_prior();
     if (p.early && tid == 0) pdl_launch_dependents();
 
     float acc[N];                                             // of the summing threads

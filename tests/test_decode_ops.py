@@ -57,6 +57,7 @@ def test_abi_refusals(lib):
     assert attend(n_requests=0) == 0
     size = lib.b200_prefix_attention_workspace_bytes
     assert size(0, 0, 8, 2, 128) == size(4, 0, 9, 2, 128) == size(4, 0, 8, 2, 80) == 0 and size(4, 0, 8, 2, 64) > 0
+    assert size(4096, 1, 64, 8, 128) < 2 ** 30                  # one group of a large batch needs no more than its tiles
 
     def int4(dtype=0, y_dtype=0, **kw):
         a = Int4()
@@ -69,7 +70,7 @@ def test_abi_refusals(lib):
 
     assert int4(y=None) == int4(x=None) == int4(codes=None) == int4(scales=None) == -1
     assert int4(dtype=2) == int4(y_dtype=1) == int4(dtype=1, y_dtype=0) == -3
-    for kw in (dict(group=16), dict(group=256), dict(n_in=224), dict(n_in=0), dict(n_out=0), dict(n_tokens=-1)):
+    for kw in (dict(group=16), dict(group=256), dict(n_in=224), dict(n_in=0), dict(n_out=0), dict(n_tokens=-1), dict(n_tokens=65535 * 32 + 1), dict(x_row=248)):
         assert int4(**kw) == -2, kw
     assert int4(x=p + 2) == int4(codes=p + 8) == int4(x_row=260) == -4
     assert int4(n_tokens=0) == 0
