@@ -129,6 +129,10 @@ __device__ __forceinline__ int worker_of_unit(long long total, long long u, int 
     return (int)quotient((u + 1) * workers - 1, total);
 }
 
+// What stands for the page of a key behind the length: never one of the cache's, but a page table can hold the same number, so whether
+// a key is there is asked of its index.
+constexpr int kNoPage = -1;
+
 __device__ __forceinline__ void cp_async16(unsigned dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }

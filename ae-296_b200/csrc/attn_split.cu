@@ -47,14 +47,13 @@ __device__ __forceinline__ unsigned chunk_addr(unsigned base, int row, int chunk
 }
 
 // The pages of the next kKeys keys of a page-table row: lane l holds key l % 16's.
-constexpr int kNoKey = -0x7fffffff - 1;
 struct PageWalk {
     const int* row;
     int keys;
 };
 __device__ __forceinline__ int page_at(const AttnParams& p, const PageWalk& w, int key0, int lane) {
     const int key = key0 + (lane & (kKeys - 1));
-    return key < w.keys ? w.row[key >> p.page_shift] : kNoKey;
+    return key < w.keys ? w.row[key >> p.page_shift] : kNoPage;
 }
 
 template <typename T, int D>
@@ -158,7 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
             if (step < n) {
                 const int key0 = (chunk0 + step) * kKeys;
                 const bool fine = page >= 0 && page < p.c.n_pages;
-                if (page != kNoKey && !fine && p.a.status) atomicOr(p.a.status, B200_DECODE_BAD_PAGE);
+                if (!fine && key0 + (lane & (kKeys - 1)) < walk.keys && p.a.status) atomicOr(p.a.status, B200_DECODE_BAD_PAGE);
                 const long long off = fine ? (long long)page * p.c.page_stride +
                                                  (long long)((key0 + (lane & 15)) & ((1 << p.page_shift) - 1)) * p.c.token_stride
                                            : -1;

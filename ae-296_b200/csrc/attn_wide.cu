@@ -58,7 +58,6 @@ struct WideShared {
     int bad, pad;
 };
 static_assert(sizeof(WideShared) % 16 == 0, "the scan's arrays follow");
-constexpr int kNoPage = -0x7fffffff - 1;         // of a key behind the prefix
 
 // one of the barrier's arrivals, once this thread's copies so far have landed
 __device__ __forceinline__ void arrive_when_copied(unsigned b) {
@@ -198,9 +197,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                 bool lost[2];
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const int key = (t.b0 + b) * kWideKeys + row_of(lane + 32 * k);
+                    const int row = row_of(lane + 32 * k), key = (t.b0 + b) * kWideKeys + row;
                     const bool fine = (unsigned)page[k] < (unsigned)p.c.n_pages;
-                    lost[k] = !fine && page[k] != kNoPage;
+                    lost[k] = !fine && row < kWideKeys && key < t.keys;
                     at[k] = fine ? (long long)page[k] * p.c.page_stride + (long long)(key & in_page) * p.c.token_stride : -1;
                 }
                 if (!is_v) {

@@ -317,6 +317,16 @@ def test_attention_leaves_bad_pages_lengths_and_groups_out_and_reports_them():
         check_attend(s, expect_status=decode.BAD_GROUPS, oracle=attend_oracle(plain))
 
 
+@pytest.mark.parametrize("value", [-2 ** 31, -1, "behind", 2 ** 31 - 1])
+@pytest.mark.parametrize("B,starts,plens", [(6, [0, 2, 5], [90, 127]), (40, [0, 39], [700])])        # groups of at most and of more than 32 rows
+def test_attention_leaves_every_page_that_does_not_exist_out(B, starts, plens, value):
+    """First, last and middle page of a row, of a request's own table and of a group's; the lowest number there is means nothing else."""
+    for name, where in (("block_table", (1, 0)), ("prefix_table", (0, 0)), ("prefix_table", (0, 3)), ("prefix_table", (0, (plens[0] - 1) // 16))):
+        s = attend_case(9, B, 8, 2, 128, 16, "bf16", [21] * B, starts=starts, plens=plens, fill=0.0)
+        s[name][where] = s["k_cache"].shape[0] if value == "behind" else value
+        check_attend(s, expect_status=decode.BAD_PAGE)
+
+
 def test_attention_without_pages_and_without_requests():
     s = attend_case(10, 4, 8, 2, 64, 16, "fp16", [0, 0, 0, 0], starts=[0, 2], plens=[40])
     s["block_table"] = s["block_table"][:, :0]
