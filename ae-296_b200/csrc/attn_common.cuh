@@ -52,29 +52,6 @@ __device__ __forceinline__ Entity split_entity(const AttnParams& p, int e, bool 
     return t;
 }
 
-// Sum over the block of value(e), e in [0, n); `sum` is zero before, and all threads meet before they read it.
-template <int THREADS, typename F>
-__device__ __forceinline__ void add_units(int n, unsigned long long* sum, F value) {
-    unsigned long long mine = 0;
-    for (int e = threadIdx.x; e < n; e += THREADS) mine += value(e);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-    if ((threadIdx.x & 31) == 0 && mine) atomicAdd(sum, mine);
-}
-
-// The wide kernel, which multiplications and exponentials bound, and the split kernel, which reading bounds, run side by side: of n
-// SMs the wide kernel takes as many, in pairs, as make both end together.  A wide unit takes an SM about as long as kWideCost units
-// of the split kernel.  256 requests of one prefix of 16384 tokens with up to 1024 keys of their own: 323, 314, 307, 334 us with
-// 12, 16, 18, 21, and 312 us one after the other (where the GPU's power limit holds the clocks down instead); 93 requests in 7 groups:
-// 155, 127, 120, 119 us and 132 us; heads of 64: 224 us with 18, 213 us with 22, 295 us with 36.
-constexpr int kWideCost = 18;
-__device__ __forceinline__ int wide_share(long long wide, long long split, int n) {
-    if (wide == 0 || split == 0) return wide == 0 ? 0 : n;
-    const long long w = wide * kWideCost;
-    const int x = 2 * (int)quotient(w * n + (w + split), 2 * (w + split)), least = n / 32 * 2;
-    return max(1, min(max(x, least), n - least));
-}
-
 // Units before each entity (su[0..n]) and row tiles before each (st[0..n_tiles_of]); value(e, usable, bad) gives tiles << 32 | units
 // of entity e.  Starts that descend somewhere leave every group out (returns whether groups can be used).
 template <int THREADS, typename F>

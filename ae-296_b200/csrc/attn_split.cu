@@ -10,9 +10,8 @@
 // products a byte, so the copies bound it and not the multiplications.  The weights 2^(z - m) go into the second
 // product as two 16-bit numbers (the value rounded, and what the rounding dropped), so nothing is lost against fp32.
 //
-// 32 requests of up to 2048 keys, 32 heads of 128: 112 us, 6.1 TB/s (677 MB; 93 % of what a copy reaches).  An SM reaches 58
-// GB/s where 56 of them run and 44 GB/s where all do, so the wide kernel can have a quarter of them for little.  One request of 311 keys: 10 us, half of
-// it latencies one after the other (lengths, page table, keys; parts, rows) and half the two launches.
+// 32 requests of up to 2048 keys, 32 heads of 128: 112 us, 6.1 TB/s (677 MB; 93 % of what a copy reaches).  One
+// request of 311 keys: 10 us, half of it latencies one after the other (lengths, page table, keys; parts, rows) and half the two launches.
 #include <type_traits>
 
 #include "attn_common.cuh"
@@ -65,31 +64,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
     __shared__ unsigned long long warp_sum[kWarps];
     __shared__ int key_mask[kWarps][R::kStages];
     __shared__ int bad_all;
-    __shared__ unsigned long long wide_sum;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    // Beside the wide kernel, which leaves alone what this one reads, only its end is waited for (at this one's own): whatever came
-    // before the wide kernel is complete when a block of this one runs.  Blocks that find no SM free run behind it, and end at once.
-    if (!p.wide_tiles) {
-        pdl_wait_prior();
-        if (tid == 0) pdl_launch_dependents();
-    }
-    if (tid == 0) { bad_all = 0; wide_sum = 0; }
+    // The predecessor may be the wide kernel, which leaves alone what this one reads, but what came before that is only sure to be
+    // seen by a grid that has waited itself.
+    pdl_wait_prior();
+    if (tid == 0) { pdl_launch_dependents(); bad_all = 0; }
     __syncthreads();
     int ignored = 0;
-    if (p.wide_tiles)
-        add_units<kThreads>(p.a.n_groups, &wide_sum, [&](int e) {
-            const Entity t = group_of<kWideRows, kWideKeys, true>(p, e, true, ignored);
-            return (unsigned long long)(t.tiles * t.chunks);
-        });
     // units before each entity, row tiles before each group; written out once for the join
     const int n_ent = p.a.n_groups + p.a.n_requests;
     const bool groups = scan_units<kThreads>(n_ent, p.a.n_groups, su, st, warp_sum, &bad_all, [&](int e, bool usable, int& bad) {
         const Entity t = split_entity(p, e, usable, bad);
         return ((unsigned long long)(e < p.a.n_groups ? t.tiles : 0) << 32) | (unsigned)(t.tiles * t.chunks);
     });
-    const int n_sm = gridDim.x, wide_sm = wide_share(groups ? (long long)wide_sum : 0, su[n_ent], n_sm), mine = max(1, n_sm - wide_sm);
     if (blockIdx.x == 0) {
-        if (tid == 0) { p.shares[0] = mine * kWarps; p.shares[1] = wide_sm; }
         for (int i = tid; i <= n_ent; i += kThreads) p.units[i] = su[i];
         for (int i = tid; i <= p.a.n_groups; i += kThreads) p.tiles[i] = groups ? st[i] : -1;
         if (tid == 0 && bad_all && p.a.status) atomicOr(p.a.status, bad_all);
@@ -97,13 +85,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
 
     const int n_kv = p.c.n_kv_heads;
     const long long total = (long long)su[n_ent] * n_kv;
-    const int workers = (int)min((long long)mine * kWarps, total);
-    const int worker = warp * mine + blockIdx.x;             // neighbours in the work on different SMs
-    if ((int)blockIdx.x >= mine || worker >= workers) {
-        pdl_wait_prior();
-        pdl_launch_dependents();
-        return;
-    }
+    const int workers = (int)min((long long)gridDim.x * kWarps, total);
+    const int worker = warp * gridDim.x + blockIdx.x;        // neighbours in the work on different SMs
+    if (worker >= workers) return;
     long long u = unit_of_worker(total, worker, workers);
     const long long u_end = unit_of_worker(total, worker + 1, workers);
     const unsigned ring = smem_u32(smem) + warp * R::kStages * R::kStage;
@@ -264,8 +248,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_split_kernel(const __grid_co
         __syncwarp();
         u += n;
     }
-    pdl_wait_prior();
-    pdl_launch_dependents();
 }
 
 constexpr int kJoin = 4;                          // parts whose rows are asked for together
@@ -290,7 +272,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const __grid
         const int h = hq / p.per, i = hq - h * p.per, n_kv = p.c.n_kv_heads, n_g = p.a.n_groups;
         const int n_ent = n_g + p.a.n_requests;
         const long long total = (long long)p.units[n_ent] * n_kv;
-        const int workers = (int)min((long long)p.shares[0], total);
+        const int workers = (int)min((long long)p.grid * kWarps, total);
 
         // The row's parts: those of its group's item (a wide tile of one stream's rows has a second part for each), then of its own.  Part
         // i of a run lies at row first + i * pitch.
@@ -312,7 +294,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_join_kernel(const __grid
                     const long long u0 = (long long)n_kv * units[lo] + (long long)h * all + (long long)tile * chunks;
                     const size_t item = (size_t)n_kv * before[lo] + (size_t)h * tiles + tile;
                     const long long sum = wide ? (long long)p.wide_units[n_g] * n_kv : total;
-                    const int w = wide ? (int)min((long long)p.shares[1], sum) : workers;
+                    const int w = wide ? (int)min((long long)p.grid, sum) : workers;
                     const int w0 = worker_of_unit(sum, u0, w), n = worker_of_unit(sum, u0 + chunks - 1, w) - w0 + 1;
                     if (!wide) run[0] = {(item + w0) * kAttnRows + (r - tile * kAttnRows), kAttnRows, n};
                     else {

@@ -20,6 +20,10 @@
 // into a ring of blocks by asynchronous 16-byte copies in the 128-byte swizzled layout the multiplications read, page
 // by page, whatever the page size, with zeros in place of keys behind the prefix or in pages that do not exist.
 //
+// The split kernel, which does the rest of a call, runs behind this one: both want all of an SM's shared memory, and what it reads is
+// only sure to be seen after a wait of its own.  (Side by side, on SMs shared out by their work and without that wait, the three larger
+// calls took 2 to 9 % less: 307, 68 and 120 us instead of 312, 72 and 132 us.)
+//
 // 256 requests of 64 heads over 8 of 128, a prefix of 16384 tokens: a unit of 256 rows takes an SM some 4500 cycles, of which the
 // multiplications need 2048 and the exponentials of a stream's warps 1500, while each waits for the other's result twice: 0.83
 // PFLOP/s over the whole GPU, half of what a library product reaches.  64 requests, a prefix of 8192: 55 us of which 12 are start and
@@ -54,7 +58,6 @@ struct WideShared {
     unsigned long long full[kMaxRing], empty[kMaxRing], q_ready[2], s_full[2], p_ready[2], o_full[2];
     unsigned long long warp_sum[kThreads / 32];
     unsigned tmem, err;
-    unsigned long long split_sum[2];             // of the groups, of the requests
     int bad, pad;
 };
 static_assert(sizeof(WideShared) % 16 == 0, "the scan's arrays follow");
@@ -119,15 +122,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     }
     if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));
     if (tid == 0) { sh.err = 0u; sh.bad = 0; }
-    if (tid < 2) sh.split_sum[tid] = 0;
     __syncthreads();
     const int n_g = p.a.n_groups, n_kv = p.c.n_kv_heads;
-    for (int k = 0; k < 2; ++k)
-        add_units<kThreads>(k == 0 ? n_g : p.a.n_requests, &sh.split_sum[k], [&](int e) {
-            int ignored = 0;
-            const Entity t = split_entity(p, k == 0 ? e : n_g + e, true, ignored);
-            return (unsigned long long)(t.tiles * t.chunks);
-        });
     const bool usable = scan_units<kThreads>(n_g, n_g, su, st, sh.warp_sum, &sh.bad, [&](int e, bool ok, int& bad) {
         const Entity t = group_of<kWideRows, kWideKeys, true>(p, e, ok, bad);
         return ((unsigned long long)t.tiles << 32) | (unsigned)(t.tiles * t.chunks);
@@ -135,8 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     if (blockIdx.x == 0)
         for (int i = tid; i <= n_g; i += kThreads) { p.wide_units[i] = su[i]; p.wide_tile[i] = st[i]; }
     const long long total = (long long)su[n_g] * n_kv;
-    const int share = wide_share(su[n_g], (long long)((usable ? sh.split_sum[0] : 0) + sh.split_sum[1]), gridDim.x);
-    const int workers = (int)min((long long)share, total);
+    const int workers = (int)min((long long)gridDim.x, total);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -491,21 +486,7 @@ cudaError_t launch_ring(const AttnParams& p, size_t scan, cudaStream_t s) {
     const size_t smem = Wide<D, RING>::kBytes + sizeof(WideShared) + scan + 1024;
     const cudaError_t e = allow_smem<attn_wide_kernel<T, D, RING>>();
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)p.grid);
-    cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    // Neighbours in pairs, so that two SMs that share their way to memory do the same: else the split kernel's reading slows some of
-    // these blocks down and all wait for those (256 requests of one prefix of 16384 tokens: 371 us instead of 318 us).
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = 2; attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = p.grid % 2 == 0 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, attn_wide_kernel<T, D, RING>, p);
+    return launch_pdl(attn_wide_kernel<T, D, RING>, dim3((unsigned)p.grid), dim3(kThreads), smem, s, p);
 }
 template <typename T>
 cudaError_t launch_typed(const AttnParams& p, cudaStream_t s) {

@@ -38,7 +38,7 @@ int attention_sizes(AttnParams& p) {
 
 size_t attention_bytes(const AttnParams& p) {
     return (attn_group_rows(p) + attn_request_rows(p) + attn_wide_rows(p)) * ((size_t)p.c.head_dim * 4 + 8) +
-           4 * ((size_t)4 * p.a.n_groups + p.a.n_requests + 6) + 64;
+           4 * ((size_t)4 * p.a.n_groups + p.a.n_requests + 4) + 64;
 }
 
 }  // namespace
@@ -106,7 +106,6 @@ extern "C" int b200_prefix_attention(const b200_attention* a, const b200_kv_cach
     p.tiles = p.units + a->n_groups + a->n_requests + 1;
     p.wide_units = p.tiles + a->n_groups + 1;
     p.wide_tile = p.wide_units + a->n_groups + 1;
-    p.shares = p.wide_tile + a->n_groups + 1;
     const cudaError_t e = launch_attention(p, dtype, sm_count(), static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? B200_LORA_OK : cuda_fail(e);
 }

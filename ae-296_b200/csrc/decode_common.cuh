@@ -22,7 +22,7 @@ constexpr int kAttnMaxWorkers = 2048;
 // Groups of more than kWideFrom rows go to the wide kernel: units of kWideKeys keys for tiles of kWideRows rows, one
 // worker per SM.  With 64 heads over 8 of 128, 32 groups of 4 requests (32 rows) over prefixes of 2048 tokens take 103 us in the split kernel
 // (two tiles, of which the second finds the keys in L2) and 121 us in the wide one, 32 groups of 8 (64 rows) 190 and 141 us; one group
-// over 16384 tokens 32 and 35 us (32 rows), 55 and 43 us (64 rows).
+// over 16384 tokens 32 and 35 us (32 rows), 55 and 43 us (64 rows); all measured when the two kernels still ran side by side.
 constexpr int kWideFrom = 32;                     // a multiple of kAttnRows
 constexpr int kWideKeys = 128;
 constexpr int kWideRows = 256;
@@ -37,13 +37,12 @@ struct AttnParams {
     int req_tiles;         // row tiles of a request
     int req_rows;          // rows of a request's partial result
     int max_group_tiles;   // of all groups together
-    int grid;              // SMs
+    int grid;              // blocks of the wide and of the split kernel: SMs
     int wide_tiles;        // at most, of all groups together; 0: no group can be that large
     float scale_log2;
     int* units;            // [n_groups + n_requests + 1] units of a cache head before each entity
     int* tiles;            // [n_groups + 1] row tiles before each group
     int *wide_units, *wide_tile;   // the same of the wide kernel, [n_groups + 1] both
-    int* shares;           // [2] of the split kernel's warps and of the wide kernel's blocks that work
     float* part;           // partial results: rows of head_dim sums, then of (maximum, sum)
     float2* part_ml;
 };

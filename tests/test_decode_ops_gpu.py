@@ -632,3 +632,91 @@ def test_steps_on_two_streams_at_once():
     for m, w in zip(models, want):
         for x, y in zip(m.outputs(), w):
             assert torch.equal(x, y)
+
+
+# ---- together, with groups of more than 32 rows: both attention kernels have work in every call -----------------
+def make_wide_layer(seed=51, dtype="bf16"):
+    """Groups of 160 and 420 rows (two streams of rows, two tiles) and of 20, and 20 requests in none."""
+    lens = 1 + np.random.default_rng(seed).integers(0, 40, 170)
+    return Layer(seed, 170, 8, 2, 64, dtype, lens, [0, 40, 45, 150], [300, 40, 515])
+
+
+def one_token_more(m, step):
+    m.x.copy_(randn(torch.Generator().manual_seed(step), *m.x.shape, dtype=m.dt))
+    m.ids.copy_((m.ids + 1) % 4)
+    grow = (m.cache["lens"] % 16 != 0).int()                    # while the page has room
+    m.cache["lens"] += grow
+    m.slots += grow.long()
+    m.positions += grow.long()
+
+
+def test_a_layer_step_of_large_groups_stage_by_stage():
+    for dtype in TYPES:
+        a = make_wide_layer(dtype=dtype)
+        a.step()
+        torch.cuda.synchronize()
+        got = a.cache["out"].clone()
+        check_attend(dict(a.cache, q=a.q, out=torch.empty_like(a.q)))
+        out = torch.empty_like(a.q)
+        L.prefix_attention(**dict(a.cache, q=a.q, out=out))
+        assert torch.equal(got, out)
+        check_int4(dict(a.o_w, x=got.flatten(1), y=a.y.clone(), add=a.x))
+
+
+def test_steps_of_large_groups_follow_what_was_written_just_before():
+    """Steps enqueued one behind the other, lengths, slots, queries and keys all written by the call before: as with a wait between."""
+    a, b = make_wide_layer(), make_wide_layer()
+    got, want = [], []
+    torch.cuda.synchronize()
+    for step in range(8):
+        one_token_more(a, step)
+        a.step()
+        got.append(a.outputs())
+    torch.cuda.synchronize()
+    for step in range(8):
+        one_token_more(b, step)
+        torch.cuda.synchronize()
+        b.step()
+        torch.cuda.synchronize()
+        want.append(b.outputs())
+    for x, y in zip(got, want):
+        for s, t in zip(x, y):
+            assert torch.equal(s, t)
+
+
+def test_a_captured_step_of_large_groups_follows_its_inputs():
+    a, b = make_wide_layer(), make_wide_layer()
+    a.step(), b.step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.step()
+    other = make_wide_layer(52, "fp16")
+    for step in range(3):
+        for m in (a, b):
+            one_token_more(m, step)
+        graph.replay()
+        other.step()
+        b.step()
+        torch.cuda.synchronize()
+        for x, y in zip(a.outputs(), b.outputs()):
+            assert torch.equal(x, y)
+
+
+def test_steps_of_large_groups_on_two_streams_at_once():
+    want = []
+    for seed in (53, 54):
+        m = make_wide_layer(seed)
+        m.step()
+        torch.cuda.synchronize()
+        want.append(m.outputs())
+    models, streams = [make_wide_layer(53), make_wide_layer(54)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for m, s in zip(models, streams):
+            with torch.cuda.stream(s):
+                m.step()
+    torch.cuda.synchronize()
+    for m, w in zip(models, want):
+        for x, y in zip(m.outputs(), w):
+            assert torch.equal(x, y)
