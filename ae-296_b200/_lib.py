@@ -70,7 +70,7 @@ class Attention(C.Structure):
 
 class Int4(C.Structure):
     _fields_ = ([(n, C.c_void_p) for n in ("y", "x", "codes", "scales", "zeros", "add")] + [(n, C.c_int64) for n in ("x_row", "y_row", "add_row")] +
-                [(n, C.c_int32) for n in ("n_tokens", "n_in", "n_out", "group")])
+                [(n, C.c_int32) for n in ("n_tokens", "n_in", "n_out", "group")] + [("status", C.c_void_p)])
 
 
 # name -> (restype, argtypes); every symbol the headers under include/ declare

@@ -30,7 +30,7 @@
 // end (queries, TMEM, the partial rows).  Tried and taken back: two threads a row (half the row each, no registers for more
 // in flight: 328 us against 314 us in all), scores kept in registers (spills: 587 us against 325 us).
 //
-// Every wait is bounded: on expiry control flow stays as it is, and the outputs become NaN.
+// Every wait is bounded: on expiry the outputs become NaN and `status` says so (tc_common.cuh).
 #include <type_traits>
 
 #include "attn_common.cuh"
@@ -57,8 +57,9 @@ struct WideShared {
     uint4 missing[kMissing][kCopyWarps];          // keys of a block in pages that do not exist, as each copy warp saw them
     unsigned long long full[kMaxRing], empty[kMaxRing], q_ready[2], s_full[2], p_ready[2], o_full[2];
     unsigned long long warp_sum[kThreads / 32];
+    unsigned long long drained;
     unsigned tmem, err;
-    int bad, pad;
+    int bad, pad[3];
 };
 static_assert(sizeof(WideShared) % 16 == 0, "the scan's arrays follow");
 
@@ -118,6 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             mbar_init(bar(sh.s_full[tid]), 1);
             mbar_init(bar(sh.o_full[tid]), 1);
         }
+        if (tid == 0) mbar_init(bar(sh.drained), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 8) tmem_alloc(smem_u32(&sh.tmem));
@@ -159,7 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
         // The page table is read a block ahead, or each copy would wait for it.
         auto row_of = [&](int i) { return (cw + kCopyWarps * (i / kRowsAt)) * kRowsAt + i % kRowsAt; };
         int page[2];
-        for (long long u = u_first; u < u_end;) {
+        bool fine = true;                        // no wait of this warp has expired
+        for (long long u = u_first; u < u_end && fine;) {
             const Part t = part_at(u);
             const int* table = p.a.prefix_table + (long long)t.g * p.a.prefix_table_row;
             auto block_at = [&](int i, bool& is_v) {
@@ -183,11 +186,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             for (int i = 0; i < 2 * t.n; ++i, ++n) {
                 if (u == u_first && i == 1) {    // the first multiplication needs the queries and one block: the others wait for those
                     for (int q = 0; q < 2; ++q)
-                        if (t.dual || q < t.n) mbar_wait(bar(sh.q_ready[q]), 0, err, 7);
+                        if (t.dual || q < t.n) fine = fine && mbar_reached(bar(sh.q_ready[q]), 0, err, 7);
                 }
                 const int slot = n % RING;
-                mbar_wait(bar(sh.empty[slot]), ((n / RING) & 1) ^ 1, err, 1);
-                __syncwarp();
+                fine = fine && mbar_reached(bar(sh.empty[slot]), ((n / RING) & 1) ^ 1, err, 1);
+                fine = __all_sync(0xffffffffu, fine);
+                if (!fine) break;
                 long long at[2];                 // < 0: zeros
                 bool lost[2];
 #pragma unroll
@@ -235,6 +239,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             u += t.n;
         }
         cp_wait_all();
+        if (cw == 0)                             // nobody else waits for the last blocks' arrivals here
+            for (unsigned i = n > RING ? n - RING : 0; i < n; ++i) fine = fine && mbar_reached(bar(sh.empty[i % RING]), (i / RING) & 1, err, 1);
     } else if (warp == 8) {
         // ================= multiplications: one thread =================
         if (lane == 0) {
@@ -243,14 +249,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
             const unsigned q0 = bar(sh.q_ready[0]), s0 = bar(sh.s_full[0]), p0 = bar(sh.p_ready[0]), o0 = bar(sh.o_full[0]);
             unsigned slot = 0, phase = 0;                        // of the block that is needed next: the ring's order is theirs
             unsigned q_phase = 0, p_phase = 0;                   // bit s: of stream s
+            bool fine = true;                                    // no wait has expired
             auto next_block = [&]() {                            // waits for it and returns its slot
                 const unsigned at = slot;
-                mbar_wait(full0 + at * 8, phase, err, 2);
+                fine = fine && mbar_reached(full0 + at * 8, phase, err, 2);
                 fence_async_proxy();                             // the copies wrote through the generic proxy
                 if (++slot == RING) { slot = 0; phase ^= 1; }
                 return at;
             };
             auto scores = [&](int s, unsigned k, bool last_use) {
+                if (!fine) return;
                 tc_fence_after();
                 const unsigned qa = q_low + s * (W::kQ >> 4), ka = desc_low(ring + k * W::kBlock, kRowsAreRows), d = tmem + s * 128;
                 mma_ss<false>(d, qa, ka, id_s);
@@ -262,10 +270,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                 tc_commit(s0 + s * 8);
                 if (last_use) tc_commit(empty0 + k * 8);
             };
-            auto queries = [&](int s) { mbar_wait(q0 + s * 8, q_phase >> s & 1, err, 3); q_phase ^= 1u << s; };
+            auto queries = [&](int s) { fine = fine && mbar_reached(q0 + s * 8, q_phase >> s & 1, err, 3); q_phase ^= 1u << s; };
             auto weigh = [&](int s, unsigned v, bool first, bool last, bool last_use) {
-                mbar_wait(p0 + s * 8, p_phase >> s & 1, err, 4);
+                fine = fine && mbar_reached(p0 + s * 8, p_phase >> s & 1, err, 4);
                 p_phase ^= 1u << s;
+                if (!fine) return;
                 tc_fence_after();
                 const unsigned va = desc_low(ring + v * W::kBlock, kRowsAreDepth), d = tmem + 256 + s * 128, w = tmem + s * 128;
                 mma_ts(d, w, va, id_o, !first);
@@ -314,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
         const float scale = fabsf(p.scale_log2);
         const float kLift = std::is_same_v<T, __half> ? 7.f : 0.f;     // fp16 weights up to 2^(8 + 7), far from its smallest numbers
         unsigned rounds = 0, outs = 0, n_keys = 0;
+        bool fine = true;                                        // no wait of this thread has expired
         for (long long u = u_first; u < u_end;) {
             const Part t = part_at(u);
             const int r_in = t.dual ? s * kStreamRows + row : row;
@@ -342,12 +352,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                         sts16(swizzled(qa, ((i0 + i) * kStreamRows + row) / kPieces, c), v[i].x ^ flip, v[i].y ^ flip, v[i].z ^ flip, v[i].w ^ flip);
                 }
                 fence_async_proxy();
-                mbar_arrive(bar(sh.q_ready[s]));
+                if (fine) mbar_arrive(bar(sh.q_ready[s]));
             }
             const bool warp_live = __ballot_sync(0xffffffffu, live) != 0u;
             float m = -INFINITY, l = 0.f;                        // sums are relative to 2^(m - kLift)
             for (int b = b_first; b < t.n; b += step, ++rounds) {
-                mbar_wait(bar(sh.s_full[s]), rounds & 1, err, 5);
+                fine = fine && mbar_reached(bar(sh.s_full[s]), rounds & 1, err, 5);
                 __syncwarp();                                    // lanes may leave a wait one by one: what follows is for whole warps
                 tc_fence_after();
                 if (warp_live) {
@@ -423,12 +433,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
                     tc_wait_st();
                 }
                 tc_fence_before();
-                mbar_arrive(bar(sh.p_ready[s]));
+                if (fine) mbar_arrive(bar(sh.p_ready[s]));
             }
             // ---- this worker's part of the rows
             const size_t out_row = t.slot + s * kStreamRows + row;
             if (b_first < t.n) {
-                mbar_wait(bar(sh.o_full[s]), outs & 1, err, 6);
+                fine = fine && mbar_reached(bar(sh.o_full[s]), outs & 1, err, 6);
                 ++outs;
                 __syncwarp();
                 tc_fence_after();
@@ -470,8 +480,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_wide_kernel(const __grid_con
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_dealloc(tmem);
-    if (sh.err) {
+    const bool lost = *reinterpret_cast<volatile unsigned*>(err) != 0u;
+    if (warp == 8) {
+        if (lost && lane == 0) {
+            tc_commit(bar(sh.drained));
+            mbar_drain(bar(sh.drained), 0);
+        }
+        __syncwarp();
+        tmem_dealloc(tmem);
+    }
+    if (lost) {
         if (tid == 0 && p.a.status) atomicOr(p.a.status, B200_DECODE_TIMEOUT);
         for (long long u = u_first; u < u_end;) {             // the join makes NaN of these
             const Part t = part_at(u);

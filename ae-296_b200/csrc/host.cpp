@@ -599,13 +599,14 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
     return PyLong_FromLong(rc);
 }
 
-// int4_linear(y, x, codes, scales, zeros, add) -> status code
+// int4_linear(y, x, codes, scales, zeros, add, status) -> status code
 PyObject* py_int4_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-    if (nargs != 6) return slow();
+    if (nargs != 7) return slow();
     Operands ops;
-    const at::Tensor* t[6];
+    const at::Tensor *t[6], *word;
     for (int i = 0; i < 6; ++i)
         if (!ops.take(args[i], i >= 4, t[i])) return slow();
+    if (!ops.take(args[6], true, word) || !int_word(word)) return slow();
     const at::Tensor &y = *t[0], &x = *t[1], &codes = *t[2], &scales = *t[3];
     int io, yd;
     if (!dtype_code(x.scalar_type(), io) || io == B200_LORA_F32 || !dtype_code(y.scalar_type(), yd) || (yd != io && yd != B200_LORA_F32)) return slow();
@@ -620,7 +621,8 @@ PyObject* py_int4_linear(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (t[4] && (t[4]->scalar_type() != at::kByte || t[4]->sizes() != scales.sizes() || !t[4]->is_contiguous())) return slow();
     if (t[5] && (t[5]->scalar_type() != y.scalar_type() || t[5]->sizes() != y.sizes() || (t[5]->stride(1) != 1 && out != 1))) return slow();
     const b200_int4 a{y.data_ptr(), x.data_ptr(), codes.data_ptr(), scales.data_ptr(), t[4] ? t[4]->data_ptr() : nullptr, t[5] ? t[5]->data_ptr() : nullptr,
-                      x.stride(0), y.stride(0), t[5] ? t[5]->stride(0) : 0, (int32_t)n, (int32_t)k, (int32_t)out, (int32_t)group};
+                      x.stride(0), y.stride(0), t[5] ? t[5]->stride(0) : 0, (int32_t)n, (int32_t)k, (int32_t)out, (int32_t)group,
+                      word ? static_cast<int32_t*>(word->data_ptr()) : nullptr};
     const c10::cuda::CUDAGuard guard((c10::DeviceIndex)ops.device);
     void* stream = stream_of(x);
     int rc;

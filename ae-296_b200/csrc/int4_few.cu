@@ -81,8 +81,9 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
     pdl_wait_prior();
     if (p.early && tid == 0) pdl_launch_dependents();
     __syncthreads();
+    int asked = min(kStages, n);                               // stages requested so far (thread 0)
     if (tid == 0)
-        for (int s = 0; s < kStages && s < n; ++s) request(s);
+        for (int s = 0; s < asked; ++s) request(s);
     // ---- factors of a chunk: a thread makes half a row's
     constexpr int kHalf = F::kGroups / 2, kChunkStages = F::kChunkStages;
     const int f_row = tid >> 1, f_first = (tid & 1) * kHalf;
@@ -119,6 +120,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
     };
     load_factors(0);
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    bool fine = true;                                          // no wait of this thread has expired
     for (int s = 0; s < n; ++s) {
         if (s % kChunkStages == 0) {
             const int chunk = s / kChunkStages;
@@ -127,11 +129,11 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
             load_factors(chunk + 1);
         }
         if (tid == 0 && s > 0 && s - 1 + kStages < n) {        // the stage before this one is soon done with by all warps
-            mbar_wait(bar(sh.empty[(s - 1) % kStages]), ((s - 1) / kStages) & 1, err, 2);
-            request(s - 1 + kStages);
+            fine = fine && mbar_reached(bar(sh.empty[(s - 1) % kStages]), ((s - 1) / kStages) & 1, err, 2);
+            if (fine) request(asked++);
         }
         const int slot = s % kStages;
-        mbar_wait(bar(sh.full[slot]), (s / kStages) & 1, err, 1);
+        fine = fine && mbar_reached(bar(sh.full[slot]), (s / kStages) & 1, err, 1);
         __syncwarp();
         const uint2* fa = factors + ((s / kChunkStages & 1) * kRows + warp * 16 + g4) * F::kPitch + (s % kChunkStages) * (kStageK / G);
         const uint2* fb = fa + 8 * F::kPitch;
@@ -178,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
             }
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar(sh.empty[slot]));
+        if (lane == 0 && fine) mbar_arrive(bar(sh.empty[slot]));
     }
     // A grid of more blocks than SMs lets a successor's come only now: earlier they would take places on the SMs that have fewer
     // blocks of this grid, and all SMs would have to wait for those (8192 columns, 32000 rows: 61 us instead of 44 us, back to back).
@@ -187,6 +189,13 @@ __global__ void __launch_bounds__(kThreads, 3) int4_few_kernel(const __grid_cons
     __syncthreads();
     float* red = reinterpret_cast<float*>(smem);
     const bool lost = *reinterpret_cast<volatile unsigned*>(err) != 0u;
+    if (lost) {
+        if (tid == 0) {
+            for (int s = max(asked - kStages, 0); s < asked; ++s) mbar_drain(bar(sh.full[s % kStages]), (s / kStages) & 1);
+            if (a.status) atomicOr(a.status, B200_DECODE_TIMEOUT);
+        }
+        __syncthreads();
+    }
     float* at = red + t4 * 2 * kRedPitch + warp * 16 + g4;
 #pragma unroll
     for (int i = 0; i < 4; ++i) at[(i & 1) * kRedPitch + (i >> 1) * 8] = lost ? __int_as_float(0x7fffffff) : acc[i];

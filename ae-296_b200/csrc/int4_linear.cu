@@ -17,7 +17,7 @@
 // blocks shares a tile's columns and its sums are added through distributed shared memory in a fixed order.
 // 8192 rows of 8192 columns, groups of 128, 64 tokens, added to y, bf16: 21 us (1.8 TB/s, 0.41 PFLOP/s; a simple mma.sync kernel took
 // 103 us): 128 blocks have 16 stages each, and turning codes into numbers bounds a stage.
-// Every wait is bounded: on expiry control flow stays as it is, and the outputs become NaN.
+// Every wait is bounded: on expiry the outputs become NaN and `status` says so (tc_common.cuh).
 #include "int4_common.cuh"
 
 namespace b200lora {
@@ -60,8 +60,9 @@ template <int G, int N> struct Shape {
     static_assert(N * kRedPitch * 4 <= kRing * kX, "the sums take x's place");
 };
 struct Int4Shared {
-    unsigned long long codes_full[8], codes_empty[8], x_full[kRing], done[kDone], a_full[6], d_empty[4];
+    unsigned long long codes_full[8], codes_empty[8], x_full[kRing], done[kDone], a_full[6], d_empty[4], drained;
     unsigned tmem, err;
+    int codes_asked, x_asked;                                 // stages of codes and blocks of x that were requested
 };
 
 template <typename T, int G, int N>
@@ -80,7 +81,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
     auto bar = [](unsigned long long& b) { return smem_u32(&b); };
     unsigned* err = &sh.err;
     const unsigned codes_at = smem_u32(smem), x_at = codes_at + S::kStages * kCodeStage;
-    auto wait_done = [&](int b, unsigned code) { if (b >= 0) mbar_wait(bar(sh.done[b % kDone]), (b / kDone) & 1, err, code); };
+    auto done = [&](int b, unsigned code) { return b < 0 || mbar_reached(bar(sh.done[b % kDone]), (b / kDone) & 1, err, code); };
 
     if (warp == kCopyWarp && lane == 0) {
         // the codes are on their way to L2 while the predecessor ends (what it may still write, L2 sees too)
@@ -90,6 +91,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
         for (int i = 0; i < kDone; ++i) mbar_init(bar(sh.done[i]), 1);
         for (int i = 0; i < S::kReady; ++i) mbar_init(bar(sh.a_full[i]), kCodeWarps / 2);
         for (int i = 0; i < S::kSums; ++i) mbar_init(bar(sh.d_empty[i]), kSumWarps);
+        mbar_init(bar(sh.drained), S::kMmaWarps);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         sh.err = 0u;
     }
@@ -111,21 +113,25 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
 
     if (warp == kCopyWarp) {
         // ================= copies of codes =================
-        if (lane == 0)
-            for (int s = 0; s < n_stages; ++s) {
+        if (lane == 0) {
+            int s = 0;
+            for (; s < n_stages; ++s) {
                 const int slot = s % S::kStages;
-                mbar_wait(bar(sh.codes_empty[slot]), ((s / S::kStages) & 1) ^ 1, err, 1);
+                if (!mbar_reached(bar(sh.codes_empty[slot]), ((s / S::kStages) & 1) ^ 1, err, 1)) break;
                 mbar_arrive_expect_tx(bar(sh.codes_full[slot]), kCodeStage);
                 tensor_g2s_2d(codes_at + slot * kCodeStage, &p.codes, (s0 + s) * (kStageK / 4), row0, bar(sh.codes_full[slot]));
             }
+            sh.codes_asked = s;
+        }
         __syncwarp();
     } else if (warp == kCopyWarp + 1) {
         // ================= copies of x =================
-        if (lane == 0)
-            for (int b = 0; b < n_blocks; ++b) {
+        if (lane == 0) {
+            int b = 0;
+            for (; b < n_blocks; ++b) {
                 const int at = b % kRing, k = s0 * kStageK + b * kBlockK;
                 const unsigned dst = x_at + at * S::kX;
-                wait_done(b - kRing, 2);
+                if (!done(b - kRing, 2)) break;
                 mbar_arrive_expect_tx(bar(sh.x_full[at]), S::kX);
                 if (p.x_panels) tensor_g2s_3d(dst, &p.x, 0, tok0, k / 64, bar(sh.x_full[at]));
                 else {
@@ -133,6 +139,8 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
                     tensor_g2s_2d(dst + S::kX / 2, &p.x, k + 64, tok0, bar(sh.x_full[at]));
                 }
             }
+            sh.x_asked = b;
+        }
         __syncwarp();
     } else if (warp >= kMmaWarp) {
         // ================= multiplications: several threads, since one cannot wait and issue as fast as the tensor core =================
@@ -140,9 +148,10 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
             const unsigned idesc = idesc_of(Cvt<T>::is_bf16, N, false);
             for (int b = warp - kMmaWarp; b < n_blocks; b += S::kMmaWarps) {
                 const int at = b % kRing, from = b % S::kNumbers, to = b % S::kSums;
-                mbar_wait(bar(sh.d_empty[to]), ((b / S::kSums) & 1) ^ 1, err, 3);
-                mbar_wait(bar(sh.x_full[at]), (b / kRing) & 1, err, 4);
-                mbar_wait(bar(sh.a_full[b % S::kReady]), (b / S::kReady) & 1, err, 5);
+                if (!mbar_reached(bar(sh.d_empty[to]), ((b / S::kSums) & 1) ^ 1, err, 3) ||
+                    !mbar_reached(bar(sh.x_full[at]), (b / kRing) & 1, err, 4) ||
+                    !mbar_reached(bar(sh.a_full[b % S::kReady]), (b / S::kReady) & 1, err, 5))
+                    break;
                 tc_fence_after();
                 const unsigned xa = desc_low(x_at + at * S::kX, kRowsAreRows);
                 const unsigned w = tmem + S::kSums * S::kSumCols + from * kACols, d = tmem + to * S::kSumCols;
@@ -186,8 +195,10 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
             for (int g = 0; g < kPer; ++g) offset[g] = zero_offset<T>(z[0] >> (8 * g) & 15u);
             z[0] = z[1]; z[1] = z[2];
             z[2] = load_zeros(s + 3);
-            mbar_wait(bar(sh.codes_full[slot]), (s / S::kStages) & 1, err, 6);
-            wait_done(b - S::kNumbers, 7);
+            // (If one of these expires, or a sum's, the tensor core multiplies what is not there yet, and y is NaN anyway.  Only a copy
+            // may not be asked for while the stage's last one is under way.)
+            mbar_reached(bar(sh.codes_full[slot]), (s / S::kStages) & 1, err, 6);
+            done(b - S::kNumbers, 7);
             __syncwarp();                                     // lanes may leave a wait one by one: what follows is for whole warps
             tc_fence_after();
             const unsigned from = codes_at + slot * kCodeStage + row * 128;
@@ -206,7 +217,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
                 }
                 tc_st16(to + q * 16, v);
             }
-            if (lane == 0) mbar_arrive(bar(sh.codes_empty[slot]));
+            if (lane == 0 && *reinterpret_cast<volatile unsigned*>(err) == 0u) mbar_arrive(bar(sh.codes_empty[slot]));
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -244,7 +255,7 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
             for (int g = 0; g < kPer; ++g) f[g] = from_bits<T>((unsigned short)((g < 2 ? sc[0].x : sc[0].y) >> (16 * (g & 1))));
             sc[0] = sc[1]; sc[1] = sc[2]; sc[2] = sc[3];
             sc[3] = load_scales(b + 4);
-            wait_done(b, 8);
+            done(b, 8);
             __syncwarp();
             tc_fence_after();
             const unsigned d = tmem + lanes + (b % S::kSums) * S::kSumCols;
@@ -265,9 +276,22 @@ __global__ void __launch_bounds__(Shape<G, N>::kThreads, N == 16 ? 2 : 1) int4_k
     if (!p.early && tid == 0) pdl_launch_dependents();                    // late, as in int4_few.cu
     // ---- sums to shared memory, where x was (all multiplications are complete: they were summed)
     __syncthreads();
+    const bool lost = *reinterpret_cast<volatile unsigned*>(err) != 0u;
+    if (lost) {
+        if (lane == 0) {
+            if (warp >= kMmaWarp) {
+                tc_commit(bar(sh.drained));
+                mbar_drain(bar(sh.drained), 0);
+            } else if (warp == kCopyWarp)
+                for (int s = max(sh.codes_asked - S::kStages, 0); s < sh.codes_asked; ++s) mbar_drain(bar(sh.codes_full[s % S::kStages]), (s / S::kStages) & 1);
+            else if (warp == kCopyWarp + 1)
+                for (int b = max(sh.x_asked - kRing, 0); b < sh.x_asked; ++b) mbar_drain(bar(sh.x_full[b % kRing]), (b / kRing) & 1);
+        }
+        if (tid == 0 && a.status) atomicOr(a.status, B200_DECODE_TIMEOUT);
+        __syncthreads();
+    }
     float* red = reinterpret_cast<float*>(smem + S::kStages * kCodeStage);
     if (warp < kSumWarps) {
-        const bool lost = *reinterpret_cast<volatile unsigned*>(err) != 0u;
 #pragma unroll
         for (int i = 0; i < N; ++i) red[i * kRedPitch + tid] = lost ? __int_as_float(0x7fffffff) : acc[i];
     }

@@ -23,6 +23,21 @@ __device__ __forceinline__ void tc_commit(unsigned bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// Bounded wait that says whether the phase is complete; on expiry it records `code`, and others then give up early.  A thread that issues
+// copies or multiplications issues no more once a wait of its has expired, and nobody whose wait has expired says that a place
+// may be filled again: so no barrier is armed while a phase of it is open.  At the end of the block, whoever issued
+// something waits for it (mbar_drain, with a limit too) before its place is used for anything else, freed, or left to the next block.
+__device__ __forceinline__ bool mbar_reached(unsigned bar, unsigned parity, unsigned* err, unsigned code) {
+    for (unsigned i = 0; i < kSpinLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 0x3ffu) == 0x3ffu && *reinterpret_cast<volatile unsigned*>(err) != 0u) return false;
+    }
+    atomicMax(err, code);
+    return false;
+}
+__device__ __forceinline__ void mbar_drain(unsigned bar, unsigned parity) {
+    for (unsigned i = 0; i < kSpinLimit && !mbar_try_wait(bar, parity); ++i) {}
+}
 // Shared-memory operands with 128-byte swizzle: panels of 64 elements, [rows][128 bytes], 16-byte piece c of row r at
 // c ^ (r % 8); 1024 bytes from one eight rows to the next.  Their descriptors as two words, of which only the low one
 // changes: address in units of 16 bytes, and above it for an operand whose rows are the contraction the distance of two panels.

@@ -150,16 +150,17 @@ def prefix_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, 
 
 
 def int4_linear(y: torch.Tensor, x: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, zeros: Optional[torch.Tensor] = None,
-                add: Optional[torch.Tensor] = None) -> None:
+                add: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
     """``y = x W^T (+ add)`` with ``W[n, k] = scales[n, k // group] * (code[n, k] - zero[n, k // group])``, for the few tokens of a decode step.
 
     ``x [T, K]``, ``y [T, N]`` (x's type, or fp32), ``codes`` uint8 ``[N, K/2]`` (column ``2i`` in the low four bits of byte ``i``, ``2i + 1`` in the high ones),
     ``scales [N, K/group]`` of x's type, ``zeros`` uint8 of the same shape (0..15; without them 8 everywhere), ``add [T, N]`` of y's type, which may be
     ``y``.  ``group`` (32, 64 or 128) follows from the shapes.  Rows of x, y and add may be strided; x and the codes start at 16-byte
-    boundaries, x's rows too.  The sums are fp32 and rounded once."""
-    rc = _lib.host().int4_linear(y, x, codes, scales, zeros, add)
+    boundaries, x's rows too.  The sums are fp32 and rounded once.  Should a wait inside the kernel run out, the outputs concerned are NaN and
+    ``TIMEOUT`` is set in ``status`` (one int32 on the device, for the caller to clear and to read)."""
+    rc = _lib.host().int4_linear(y, x, codes, scales, zeros, add, status)
     if rc > 0:
-        _same_device("int4_linear", (y, x, codes, scales), (zeros, add))
+        _same_device("int4_linear", (y, x, codes, scales), (zeros, add, status))
         _refuse("int4_linear", [
             (lambda: x.dim() == 2 and y.dim() == 2 and codes.dim() == 2 and scales.dim() == 2, "x, y, codes and scales must be matrices"),
             (lambda: x.dtype in (torch.float16, torch.bfloat16), "x must be fp16 or bf16"),
@@ -172,5 +173,6 @@ def int4_linear(y: torch.Tensor, x: torch.Tensor, codes: torch.Tensor, scales: t
             (lambda: codes.is_contiguous() and scales.is_contiguous(), "codes and scales must be contiguous"),
             (lambda: zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape and zeros.is_contiguous()),
              "zeros must be contiguous uint8 of the scales' shape"),
-            (lambda: add is None or (add.dtype == y.dtype and add.shape == y.shape and add.stride(1) == 1), "add must have y's shape and type")])
+            (lambda: add is None or (add.dtype == y.dtype and add.shape == y.shape and add.stride(1) == 1), "add must have y's shape and type"),
+            _status_test(status)])
     check(rc, "int4_linear")

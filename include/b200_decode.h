@@ -27,7 +27,8 @@ enum {
     B200_DECODE_BAD_LENGTH = 8,    /* attention: a negative length, or one longer than the row of the page table; it
                                       was taken as zero, or as the row's */
     B200_DECODE_BAD_GROUPS = 16,   /* attention: group starts that descend or lie outside the batch; no prefix was used */
-    B200_DECODE_TIMEOUT = 32       /* attention: a bounded wait inside a kernel expired; the outputs concerned are NaN */
+    B200_DECODE_TIMEOUT = 32       /* attention, 4-bit products: a bounded wait inside a kernel expired; the outputs
+                                      concerned are NaN */
 };
 enum { B200_DECODE_MAX_REQUESTS = 4096, B200_DECODE_MAX_GROUPS = 2048 };
 
@@ -102,6 +103,7 @@ typedef struct b200_int4 {
     const void *x, *codes, *scales, *zeros, *add;
     int64_t x_row, y_row, add_row;
     int32_t n_tokens, n_in, n_out, group;
+    int32_t* status;
 } b200_int4;
 int b200_int4_linear(const b200_int4* a, int32_t dtype, int32_t y_dtype, void* stream);
 

@@ -159,3 +159,30 @@ def test_oracle_identities():
         np.testing.assert_allclose(w, s)
     codes = np.array([[0x21, 0xF0]], np.uint8)
     np.testing.assert_array_equal(O.int4_weights(codes, np.array([[2.0]])), [[-14.0, -12.0, -16.0, 14.0]])
+
+
+def test_int4_takes_a_status_word_and_refuses_others(lib):
+    import ae296_b200 as L
+    good = dict(y=fake(3, 40), x=fake(3, 256), codes=fake(40, 128, dtype=torch.uint8), scales=fake(40, 4))
+    for word in (fake(1, dtype=I64), fake(2, dtype=I32), fake(1, dtype=F32), torch.zeros(1, dtype=I32)):
+        with pytest.raises(ValueError):
+            L.int4_linear(**good, status=word)
+
+
+def test_structures_have_the_header_s_sizes(tmp_path):
+    """The ctypes structures against the C compiler's."""
+    import os
+    import shutil
+    import subprocess
+    from ae296_b200 import _lib
+    cc = shutil.which("gcc") or shutil.which("cc")
+    if cc is None:
+        pytest.skip("no C compiler")
+    pairs = [("b200_kv_cache", _lib.KvCache), ("b200_append", _lib.Append), ("b200_attention", _lib.Attention), ("b200_int4", _lib.Int4)]
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "b200_decode.h"\nint main(void) {\n' + "".join(
+        f'    printf("%zu\\n", sizeof({c}));\n' + "".join(f'    printf("%zu\\n", offsetof({c}, {n}));\n' for n, _ in t._fields_) for c, t in pairs) + "    return 0;\n}\n")
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run([cc, "-I", include, str(src), "-o", str(tmp_path / "sizes")], check=True)
+    got = [int(x) for x in subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.split()]
+    assert got == [x for _, t in pairs for x in (C.sizeof(t), *(getattr(t, n).offset for n, _ in t._fields_))]

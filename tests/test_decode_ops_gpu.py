@@ -480,6 +480,16 @@ def test_int4_infinite_and_nan_inputs_stay_in_their_token():
     assert torch.isnan(s["y"][8]).all() and not torch.isfinite(s["y"][3]).any()
 
 
+@pytest.mark.parametrize("T", [1, 2, 3, 8, 9, 33, 64])
+def test_int4_leaves_a_status_word_alone(T):
+    """Nothing but an expired wait writes to it; what other calls have set stays."""
+    s = int4_case(T, T, 512, 200, 64, "bf16")
+    for value in (0, decode.BAD_PAGE):
+        word = torch.full((1,), value, dtype=torch.int32, device="cuda")
+        check_int4(dict(s, status=word))
+        assert int(word) == value
+
+
 # ---- together --------------------------------------------------------------------------------------
 class Layer:
     """A decode layer's attention block with 4-bit projections and deltas; every stage's output is kept."""
