@@ -23,6 +23,7 @@
 
 #include <string.h>
 
+#include <cmath>
 #include <memory>
 #include <mutex>
 #include <vector>
@@ -542,7 +543,7 @@ PyObject* py_append_kv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     return PyLong_FromLong(rc);
 }
 
-// prefix_attention(out, q, k_cache, v_cache, block_table, lens, prefix_table, prefix_lens, group_starts, scale, lse, status)
+// prefix_attention(out, q, k_cache, v_cache, block_table, lens, prefix_table, prefix_lens, group_starts, scale | None, lse, status)
 // -> status code.  The workspace comes from torch's allocator for the call, so it belongs to the stream or to the
 // graph that is being captured.
 PyObject* py_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -552,7 +553,7 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
     for (int i = 0; i < 9; ++i)
         if (!ops.take(args[i], i >= 6, t[i])) return slow();
     if (!ops.take(args[10], true, lse) || !ops.take(args[11], true, word) || !int_word(word)) return slow();
-    const double scale = PyFloat_AsDouble(args[9]);
+    const double scale = args[9] == Py_None ? 0.0 : PyFloat_AsDouble(args[9]);
     if (PyErr_Occurred()) return slow();
     const at::Tensor &out = *t[0], &q = *t[1], &table = *t[4], &lens = *t[5];
     b200_kv_cache c;
@@ -569,7 +570,7 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
     b200_attention a;
     memset(&a, 0, sizeof(a));
     if (t[6] || t[7] || t[8]) {
-        if (!t[6] || !t[7] || !t[8]) return slow();
+        if (!t[6] || !t[7] || !t[8] || t[6]->dim() != 2) return slow();
         const int64_t g = t[6]->size(0);
         if (!fits_int(g) || !table_of(*t[6], g) || !vector_of(*t[7], g) || !vector_of(*t[8], g + 1) || t[7]->scalar_type() != at::kInt ||
             t[8]->scalar_type() != at::kInt)
@@ -583,7 +584,7 @@ PyObject* py_prefix_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs
     a.q_row = q.stride(0); a.q_head = q.stride(1); a.out_row = out.stride(0); a.out_head = out.stride(1);
     a.table = static_cast<const int32_t*>(table.data_ptr()); a.table_row = table.stride(0); a.max_pages = (int32_t)table.size(1);
     a.lens = static_cast<const int32_t*>(lens.data_ptr());
-    a.n_requests = (int32_t)b; a.n_heads = (int32_t)hq; a.scale = (float)scale;
+    a.n_requests = (int32_t)b; a.n_heads = (int32_t)hq; a.scale = (float)(args[9] == Py_None ? std::pow((double)d, -0.5) : scale);
     a.status = word ? static_cast<int32_t*>(word->data_ptr()) : nullptr;
     if (b == 0) return PyLong_FromLong(0);
     const size_t bytes = b200_prefix_attention_workspace_bytes((int32_t)b, a.n_groups, (int32_t)hq, c.n_kv_heads, c.head_dim);

@@ -119,8 +119,7 @@ def prefix_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, 
     influence.  Lengths and tables stay on the device; a page outside the cache is left out, a length outside its table is cut,
     group starts that do not ascend inside the batch leave all prefixes out; each sets its bit (``BAD_PAGE``, ``BAD_LENGTH``,
     ``BAD_GROUPS``; ``TIMEOUT`` if a wait inside the kernel ran out) in ``status`` (one int32 on the device, for the caller to clear and to read).  At most 4096 requests and 2048 groups."""
-    rc = _lib.host().prefix_attention(out, q, k_cache, v_cache, block_table, lens, prefix_table, prefix_lens, group_starts,
-                                      q.shape[-1] ** -0.5 if scale is None else scale, lse, status)
+    rc = _lib.host().prefix_attention(out, q, k_cache, v_cache, block_table, lens, prefix_table, prefix_lens, group_starts, scale, lse, status)
     if rc > 0:
         _same_device("prefix_attention", (out, q, k_cache, v_cache, block_table, lens), (prefix_table, prefix_lens, group_starts, lse, status))
         given = [x is not None for x in (prefix_table, prefix_lens, group_starts)]
@@ -135,7 +134,8 @@ def prefix_attention(out: torch.Tensor, q: torch.Tensor, k_cache: torch.Tensor, 
             (lambda: block_table.dim() == 2 and block_table.shape[0] == q.shape[0] and (block_table.stride(1) == 1 or block_table.shape[1] <= 1),
              "block_table must be [requests, pages] with contiguous rows"),
             (lambda: lens.dim() == 1 and lens.shape[0] == q.shape[0] and lens.is_contiguous(), "lens must be contiguous [requests]"),
-            (lambda: all(given) or not any(given), "prefix_table, prefix_lens and group_starts go together")]
+            (lambda: all(given) or not any(given), "prefix_table, prefix_lens and group_starts go together"),
+            (lambda: scale is None or hasattr(scale, "__float__"), "scale must be a number")]
         if all(given):
             tests += [
                 (lambda: prefix_table.dim() == 2 and prefix_table.shape[0] <= 2048, "at most 2048 groups"),

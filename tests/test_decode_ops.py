@@ -169,6 +169,18 @@ def test_int4_takes_a_status_word_and_refuses_others(lib):
             L.int4_linear(**good, status=word)
 
 
+def test_attention_names_what_is_wrong_with_odd_arguments(lib):
+    """What has no shape, or not the dimensions that the default scale and the number of groups are read from."""
+    import ae296_b200 as L
+    good = dict(out=fake(4, 8, 64), q=fake(4, 8, 64), k_cache=fake(5, 16, 2, 64), v_cache=fake(5, 16, 2, 64), block_table=fake(4, 3, dtype=I32), lens=fake(4, dtype=I32))
+    pre = dict(prefix_table=fake(2, 3, dtype=I32), prefix_lens=fake(2, dtype=I32), group_starts=fake(3, dtype=I32))
+    for kw, why in ((dict(q=None), "tensors expected"), (dict(q=[1.0]), "tensors expected"), (dict(q=fake(()), out=fake(())), "q must be"),
+                    (dict(q=fake(4, 8, 0), out=fake(4, 8, 0)), "head_dim"), (dict(pre, prefix_table=fake((), dtype=I32)), "groups"),
+                    (dict(pre, prefix_table=fake(2, dtype=I32)), "groups"), (dict(scale="0.1"), "number")):
+        with pytest.raises(ValueError, match=why):
+            L.prefix_attention(**dict(good, **kw))
+
+
 def test_structures_have_the_header_s_sizes(tmp_path):
     """The ctypes structures against the C compiler's."""
     import os
