@@ -115,6 +115,7 @@ extern "C" int b200_int4_linear(const b200_int4* a, int32_t dtype, int32_t y_dty
     if (!io_type(dtype) || (y_dtype != dtype && y_dtype != B200_LORA_F32)) return B200_LORA_ERR_DTYPE;
     if (a->n_tokens < 0 || a->n_in < 1 || a->n_out < 1 || (a->group != 32 && a->group != 64 && a->group != 128) || a->n_in % a->group != 0)
         return B200_LORA_ERR_DIM;
+    if (a->n_in > 0x7fffff00 || a->n_out > 0x7fffff00) return B200_LORA_ERR_DIM;       // rounded up to whole tiles they are 32-bit numbers
     if (!aligned16(a->x) || !aligned16(a->codes) || (a->n_tokens > 1 && a->x_row % 8 != 0)) return B200_LORA_ERR_ALIGN;
     if (a->n_tokens == 0) return B200_LORA_OK;
     b200_int4 q = *a;

@@ -97,7 +97,7 @@ int b200_prefix_attention(const b200_attention* a, const b200_kv_cache* cache, i
  * scales [n_out, n_in / group] of x's type; zeros (NULL: 8 everywhere) [n_out, n_in / group] bytes, of which the low
  * four bits count; both contiguous.  group is 32, 64 or 128 and divides n_in.  x [n_tokens, n_in] and y
  * [n_tokens, n_out] with row strides (x's rows do not overlap); y and add are of x's type or both fp32; add (NULL: none) may be y.  Made for the
- * few tokens of a decode step; at most 65535 * 32 of them. */
+ * few tokens of a decode step; at most 65535 * 32 of them, and at most 2^31 - 256 inputs and outputs. */
 typedef struct b200_int4 {
     void* y;
     const void *x, *codes, *scales, *zeros, *add;

@@ -161,6 +161,17 @@ def test_oracle_identities():
     np.testing.assert_array_equal(O.int4_weights(codes, np.array([[2.0]])), [[-14.0, -12.0, -16.0, 14.0]])
 
 
+def test_int4_refuses_sizes_that_do_not_round_up_in_32_bits(lib):
+    from ae296_b200._lib import Int4
+    for kw in (dict(n_in=2 ** 31 - 128), dict(n_in=2 ** 31 - 32, group=32), dict(n_out=2 ** 31 - 255), dict(n_out=2 ** 31 - 1), dict(n_out=2 ** 31 - 1, n_tokens=40)):
+        a = Int4()
+        a.y = a.x = a.codes = a.scales = 1 << 20
+        a.x_row, a.y_row, a.n_tokens, a.n_in, a.n_out, a.group = 2 ** 31, 2 ** 31, 2, 256, 64, 64
+        for n, v in kw.items():
+            setattr(a, n, v)
+        assert lib.b200_int4_linear(C.byref(a), 0, 0, None) == -2, kw
+
+
 def test_int4_takes_a_status_word_and_refuses_others(lib):
     import ae296_b200 as L
     good = dict(y=fake(3, 40), x=fake(3, 256), codes=fake(40, 128, dtype=torch.uint8), scales=fake(40, 4))
