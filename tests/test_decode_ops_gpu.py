@@ -327,6 +327,34 @@ def test_attention_leaves_every_page_that_does_not_exist_out(B, starts, plens, v
         check_attend(s, expect_status=decode.BAD_PAGE)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 1)])
+def test_attention_of_small_groups_has_the_weights_in_full(d, page, dtype):
+    """Groups of at most 32 rows, like own keys, take each weight as two 16-bit numbers: its error is that of the exponent, of the exponential and
+    h^2, not h.  Values around zero leave many outputs so small that their own rounding hides nothing."""
+    s = attend_case(13, 24, 8, 2, d, page, dtype, [1, 0, 2, 5] * 6, starts=[0, 8, 12, 13, 21], plens=[40, 17, 33, 24], std=0.3)
+    s["v_cache"] -= 0.25
+    want, lse, weighted = attend_oracle(s)
+    L.prefix_attention(**s)
+    dt, h = s["q"].dtype, half_step(s["q"].dtype)
+    zmax = d ** -0.5 * float(s["q"].float().norm(dim=-1).max()) * float(torch.nan_to_num(s["k_cache"].float()).norm(dim=-1).max())
+    weight = (d + 4) * 2 * U * zmax + 4 * U + h * h
+    within(f64(s["out"]), want, h * np.abs(want) + weighted * (2 * weight + 2 * U * 45) + tiny(dt), "out")
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("B,starts,plens", [(7, [0, 2, 7], [90, 127]), (60, [0, 37, 59], [300, 129])])       # groups of at most and of more than 32 rows
+def test_attention_no_bit_depends_on_what_lies_behind_the_lengths(B, starts, plens, dtype):
+    outs = []
+    for fill in (0.0, float("nan"), float("inf"), -float("inf"), 60000.0):
+        s = attend_case(14, B, 8, 2, 128, 64, dtype, [(7 * i) % 70 for i in range(B)], starts=starts, plens=plens, fill=fill)
+        lse = torch.empty(B, 8, device="cuda")
+        L.prefix_attention(**s, lse=lse)
+        outs.append((s["out"], lse))
+    for out, lse in outs[1:]:
+        assert torch.equal(out, outs[0][0]) and torch.equal(lse, outs[0][1])
+
+
 def test_attention_without_pages_and_without_requests():
     s = attend_case(10, 4, 8, 2, 64, 16, "fp16", [0, 0, 0, 0], starts=[0, 2], plens=[40])
     s["block_table"] = s["block_table"][:, :0]
