@@ -14,7 +14,8 @@
 //
 // The running maximum is not followed exactly: the sums are only rescaled when a row's maximum has grown by more than
 // 2^8, since fp32 sums and 16-bit weights up to 256 lose nothing by a common factor.  P is rounded to the 16-bit type
-// (relative 2^-9 or 2^-12, as often up as down): what the output's own rounding does again.
+// (by up to 2^-8 or 2^-11 of its size, as often up as down): what the output's own rounding does again.  The sum of the weights
+// takes them as they were, so lse does not feel that rounding and a row's weights sum to one only up to it.
 //
 // Warps 0..3 and 4..7: the streams.  Warp 8: one thread issues the multiplications.  Warps 9..11 bring keys and values
 // into a ring of blocks by asynchronous 16-byte copies in the 128-byte swizzled layout the multiplications read, page

@@ -6,10 +6,11 @@
 // as it is by the multiply-add of 16-bit factors and an fp32 sum, so that x needs no conversion.  x lies in shared memory in the
 // order in which lanes ask for it.  Where rows are few a block's warps share their columns.
 //
-// Some 2.3 instructions a code bound it, of which 0.75 go through the integer pipe (with fp32 numbers made by permutations 2.1 did: 45 us
-// instead of 40 us for 32000 rows of 8192 columns).  One token, bf16, back to back: 4096 rows of 4096 columns 4.7 us, 1024 of 8192
-// 3.7 us, 8192 of 8192 12.1 us (2.9 TB/s), 32000 of 8192 40.1 us (3.6 TB/s).  Rows shared out evenly among the warps instead of four at a
-// time: 5.2, 3.9, 13.5, 42.7 us; three blocks an SM: 6.6, 4.8, 18.9, 46.1 us.
+// This way of doing it takes some 2.3 instructions a code, which bound it (for 32000 rows of 8192 columns the bytes would take 22 us);
+// 0.75 of them go through the integer pipe (with fp32 numbers made by permutations 2.1 did: 45 us instead of 40 us for those rows).  One
+// token, bf16, back to back: 4096 rows of 4096 columns 4.7 us, 1024 of 8192 3.7 us, 8192 of 8192 12.1 us (2.9 TB/s), 32000 of 8192 40.1 us
+// (3.6 TB/s).  Rows shared out evenly among the warps instead of four at a time: 5.2, 3.9, 13.5, 42.7 us; three blocks an SM: 6.6, 4.8, 18.9,
+// 46.1 us.
 #include "int4_common.cuh"
 
 namespace b200lora {
